@@ -446,6 +446,127 @@ int hodu_rocm_attention_masked(hodu_rocm_ctx *ctx, int dtype, const void *q, con
     return attention_entry(ctx, dtype, q, k, v, out, md, len, scale, causal, mask, mask_dtype, mask_layout, mask_layout_len, true);
 }
 
+// the scalar `scale` of dtype bf16 / f16, widened; false for another dtype
+static bool widened_scale(int dtype, const void *scale, float *out) {
+    if (dtype == HODU_BF16) {
+        uint16_t h;
+        memcpy(&h, scale, 2);
+        uint32_t u = (uint32_t)h << 16;
+        memcpy(out, &u, 4);
+        return true;
+    }
+    if (dtype == HODU_F16) {
+        _Float16 h;
+        memcpy(&h, scale, 2);
+        *out = (float)h;
+        return true;
+    }
+    return false;
+}
+
+// an 8-bit cache comes with scales, a 16-bit one of the operands' type without
+static int check_cache_dtype(const char *what, int dtype, int cache_dtype, const void *k_scale, const void *v_scale) {
+    if (dtype != HODU_BF16 && dtype != HODU_F16) return fail(HODU_ROCM_UNSUPPORTED, "%s: takes bf16 and f16 (dtype id %d)", what, dtype);
+    if (cache_dtype != dtype && cache_dtype != HODU_F8E4M3)
+        return fail(HODU_ROCM_UNSUPPORTED, "%s: the cache is of the operands' dtype or f8e4m3 (dtype id %d)", what, cache_dtype);
+    if (cache_dtype == HODU_F8E4M3 && (!k_scale || !v_scale))
+        return fail(HODU_ROCM_INVALID_ARG, "%s: an f8e4m3 cache needs a scale per key / value head (k_scale, v_scale)", what);
+    if (cache_dtype != HODU_F8E4M3 && (k_scale || v_scale))
+        return fail(HODU_ROCM_INVALID_ARG, "%s: scales come with an f8e4m3 cache only", what);
+    return HODU_ROCM_OK;
+}
+
+int hodu_rocm_paged_plan(hodu_rocm_ctx *ctx, const int *cached, const int *added, const int *free_pages, int *table, int *lens,
+                         int *offsets, int *slots, int *used, const size_t *md, size_t len) {
+    clear_error();
+    if (!ctx) return fail(HODU_ROCM_INVALID_ARG, "paged_plan: context is null");
+    PagedPlanArgs a;
+    int rc = parse_paged_plan_metadata(md, len, &a);
+    if (rc) return rc;
+    if (!offsets || !used) return fail(HODU_ROCM_INVALID_ARG, "paged_plan: null pointer");
+    if (a.batch > 0 && (!cached || !added || !lens || (!table && a.width > 0))) return fail(HODU_ROCM_INVALID_ARG, "paged_plan: null pointer");
+    if ((!free_pages && a.n_free > 0) || (!slots && a.capacity > 0)) return fail(HODU_ROCM_INVALID_ARG, "paged_plan: null pointer");
+    const void *outs[5] = {table, lens, offsets, slots, used}, *ins[3] = {cached, added, free_pages};
+    for (int i = 0; i < 5; i++) {
+        for (int j = 0; j < 3; j++)
+            if (outs[i] && outs[i] == ins[j]) return fail(HODU_ROCM_INVALID_ARG, "paged_plan: an output aliases an input");
+        for (int j = i + 1; j < 5; j++)
+            if (outs[i] && outs[i] == outs[j]) return fail(HODU_ROCM_INVALID_ARG, "paged_plan: two outputs are the same memory");
+    }
+    std::lock_guard<std::recursive_mutex> hold(ctx->mu);
+    HODU_HIP(hipSetDevice(ctx->device));
+    return launch_paged_plan(ctx, cached, added, free_pages, table, lens, offsets, slots, used, a);
+}
+
+int hodu_rocm_paged_store(hodu_rocm_ctx *ctx, int dtype, int cache_dtype, const void *k, const void *v, void *k_cache, void *v_cache,
+                          const int *slots, const float *k_scale, const float *v_scale, const size_t *md, size_t len) {
+    clear_error();
+    if (!ctx) return fail(HODU_ROCM_INVALID_ARG, "paged_store: context is null");
+    if (!k || !v || !k_cache || !v_cache || !slots) return fail(HODU_ROCM_INVALID_ARG, "paged_store: null pointer");
+    if (k_cache == k || k_cache == v || v_cache == k || v_cache == v)
+        return fail(HODU_ROCM_INVALID_ARG, "paged_store: the cache aliases an input");
+    PagedStoreArgs a;
+    int rc = parse_paged_store_metadata(md, len, &a);
+    if (rc) return rc;
+    rc = check_cache_dtype("paged_store", dtype, cache_dtype, k_scale, v_scale);
+    if (rc) return rc;
+    if (a.tokens == 0 || a.kv_heads == 0 || a.d == 0 || a.n_pages == 0) return HODU_ROCM_OK;
+    std::lock_guard<std::recursive_mutex> hold(ctx->mu);
+    HODU_HIP(hipSetDevice(ctx->device));
+    rc = launch_paged_store(ctx, dtype, cache_dtype, k, v, k_cache, v_cache, slots, k_scale, v_scale, a);
+    if (rc == HODU_ROCM_UNSUPPORTED)
+        return fail(HODU_ROCM_UNSUPPORTED, "paged_store: needs a head dim, strides, offsets and bases that are multiples of 8 elements");
+    return rc;
+}
+
+static int seq_attention_entry(const char *what, hodu_rocm_ctx *ctx, int dtype, int cache_dtype, const void *q, const void *k, const void *v,
+                               void *out, const void *scale, SeqAttentionArgs &a) {
+    if (!widened_scale(dtype, scale, &a.scale)) return fail(HODU_ROCM_UNSUPPORTED, "%s: takes bf16 and f16 (dtype id %d)", what, dtype);
+    if (a.batch == 0 || a.q_tokens == 0) return HODU_ROCM_OK;
+    std::lock_guard<std::recursive_mutex> hold(ctx->mu);
+    HODU_HIP(hipSetDevice(ctx->device));
+    int rc = launch_seq_attention(ctx, dtype, cache_dtype, q, k, v, out, a);
+    if (rc == HODU_ROCM_UNSUPPORTED)
+        return fail(HODU_ROCM_UNSUPPORTED, "%s: needs head dim 64 or 128, 16-byte aligned rows, heads and bases and a positive finite scale", what);
+    return rc;
+}
+
+int hodu_rocm_attention_varlen(hodu_rocm_ctx *ctx, int dtype, const void *q, const void *k, const void *v, void *out, const int *q_offsets,
+                               const int *k_offsets, const size_t *md, size_t len, const void *scale, int causal) {
+    clear_error();
+    if (!ctx) return fail(HODU_ROCM_INVALID_ARG, "attention_varlen: context is null");
+    if (!q || !k || !v || !out || !q_offsets || !k_offsets || !scale) return fail(HODU_ROCM_INVALID_ARG, "attention_varlen: null pointer");
+    if (out == q || out == k || out == v) return fail(HODU_ROCM_INVALID_ARG, "attention_varlen: out aliases an input");
+    SeqAttentionArgs a;
+    int rc = parse_varlen_metadata(md, len, &a);
+    if (rc) return rc;
+    a.q_offsets = q_offsets;
+    a.k_offsets = k_offsets;
+    a.causal = causal != 0;
+    return seq_attention_entry("attention_varlen", ctx, dtype, dtype, q, k, v, out, scale, a);
+}
+
+int hodu_rocm_attention_paged(hodu_rocm_ctx *ctx, int dtype, int cache_dtype, const void *q, const void *k_cache, const void *v_cache, void *out,
+                              const int *q_offsets, const int *table, const int *lens, const float *k_scale, const float *v_scale,
+                              const size_t *md, size_t len, const void *scale) {
+    clear_error();
+    if (!ctx) return fail(HODU_ROCM_INVALID_ARG, "attention_paged: context is null");
+    if (!q || !k_cache || !v_cache || !out || !q_offsets || !table || !lens || !scale)
+        return fail(HODU_ROCM_INVALID_ARG, "attention_paged: null pointer");
+    if (out == q || out == k_cache || out == v_cache) return fail(HODU_ROCM_INVALID_ARG, "attention_paged: out aliases an input");
+    SeqAttentionArgs a;
+    int rc = parse_paged_attention_metadata(md, len, &a);
+    if (rc) return rc;
+    rc = check_cache_dtype("attention_paged", dtype, cache_dtype, k_scale, v_scale);
+    if (rc) return rc;
+    a.q_offsets = q_offsets;
+    a.table = table;
+    a.lens = lens;
+    a.k_scale = k_scale;
+    a.v_scale = v_scale;
+    return seq_attention_entry("attention_paged", ctx, dtype, cache_dtype, q, k_cache, v_cache, out, scale, a);
+}
+
 int hodu_rocm_contiguous(hodu_rocm_ctx *ctx, int dtype, const void *in, void *out, const size_t *md, size_t len) {
     clear_error();
     if (!ctx) return fail(HODU_ROCM_INVALID_ARG, "contiguous: context is null");

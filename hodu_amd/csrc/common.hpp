@@ -252,6 +252,67 @@ struct AttentionMask {
 int launch_attention(hodu_rocm_ctx *ctx, int dtype, const void *q, const void *k, const void *v, void *out,
                      const AttentionArgs &a, const AttentionMask *mask = nullptr);
 
+// Division of a non-negative 31-bit index by a fixed extent as a multiplication: n / d = n * mul >> sh with
+// sh = 31 + ceil(log2 d) and mul = ceil(2^sh / d).  Exact: mul * d = 2^sh + e with e < d <= 2^(sh - 31), so the excess
+// n * e / (d * 2^sh) stays below 1 / d for n < 2^31.
+struct FixedDiv {
+    unsigned long long mul = 1;
+    int d = 1, sh = 0;
+};
+inline FixedDiv fixed_div(int d) {
+    FixedDiv f;
+    int up = 0;
+    while ((1LL << up) < d) up++;
+    f.d = d;
+    f.sh = 31 + up;
+    f.mul = ((1ULL << f.sh) + (unsigned long long)d - 1) / (unsigned long long)d;
+    return f;
+}
+
+// The paged cache of keys and values (one of the two): page p, token t of the page, kv head h, element e at
+// off + p * page + t * token + h * head + e.  Element strides.
+struct PagedSide {
+    long page = 0, token = 0, head = 0, off = 0;
+};
+// block tables and slot maps from request lengths (paged.hip)
+struct PagedPlanArgs {
+    long batch = 0, page_size = 0, width = 0, n_free = 0, capacity = 0;
+};
+int parse_paged_plan_metadata(const size_t *md, size_t len, PagedPlanArgs *a);
+int launch_paged_plan(hodu_rocm_ctx *ctx, const int *cached, const int *added, const int *free_pages, int *table, int *lens,
+                      int *offsets, int *slots, int *used, const PagedPlanArgs &a);
+// new keys and values into their slots of the cache (paged.hip)
+struct PagedStoreArgs {
+    long tokens = 0, kv_heads = 0, d = 0, n_pages = 0, page_size = 0;
+    long k_token = 0, k_head = 0, k_off = 0, v_token = 0, v_head = 0, v_off = 0;
+    PagedSide kc, vc;
+};
+int parse_paged_store_metadata(const size_t *md, size_t len, PagedStoreArgs *a);
+int launch_paged_store(hodu_rocm_ctx *ctx, int dtype, int cache_dtype, const void *k, const void *v, void *k_cache, void *v_cache,
+                       const int *slots, const float *k_scale, const float *v_scale, const PagedStoreArgs &a);
+// attention of packed sequences of different lengths with grouped heads (attention_seq.hip): keys packed like the
+// queries (paged == false: kc / vc hold token and head strides, k_offsets the sequences' first tokens) or in the pages
+// of a cache
+struct SeqAttentionArgs {
+    long batch = 0, q_tokens = 0, heads = 0, kv_heads = 0, d = 0;
+    long q_token = 0, q_head = 0, q_off = 0;
+    PagedSide kc, vc;
+    bool paged = false;
+    long k_tokens = 0;                         // packed keys
+    long n_pages = 0, page_size = 1, width = 0;  // paged keys: pages of the cache, tokens of a page, table columns
+    const int *q_offsets = nullptr;            // [batch + 1]
+    const int *k_offsets = nullptr;            // [batch + 1], packed keys
+    const int *table = nullptr, *lens = nullptr;  // [batch, width], [batch]: paged keys
+    const float *k_scale = nullptr, *v_scale = nullptr;  // [kv_heads], an 8-bit cache
+    float scale = 1.f;
+    bool causal = false;
+};
+int parse_varlen_metadata(const size_t *md, size_t len, SeqAttentionArgs *a);
+int parse_paged_attention_metadata(const size_t *md, size_t len, SeqAttentionArgs *a);
+// HODU_ROCM_UNSUPPORTED without an error text when no kernel takes the call
+int launch_seq_attention(hodu_rocm_ctx *ctx, int dtype, int cache_dtype, const void *q, const void *k, const void *v, void *out,
+                         const SeqAttentionArgs &a);
+
 int launch_cast(hodu_rocm_ctx *ctx, int src, int dst, const void *in, void *out, const Strided &s);
 int launch_gather(hodu_rocm_ctx *ctx, int dtype, const void *in, void *out, const Strided &s);
 

@@ -234,4 +234,95 @@ int parse_attention_metadata(const size_t *md, size_t len, AttentionArgs *a) {
     return HODU_ROCM_OK;
 }
 
+namespace {
+constexpr size_t kMaxInt = 0x7FFFFFFF;
+// a metadata vector of exactly `want` words, each in range
+int check_words(const char *what, const size_t *md, size_t len, size_t want) {
+    if (!md) return fail(HODU_ROCM_INVALID_ARG, "%s: metadata is null", what);
+    if (len != want) return fail(HODU_ROCM_INVALID_ARG, "%s: metadata has %zu words, expected %zu", what, len, want);
+    for (size_t i = 0; i < len; i++)
+        if (!sane(md[i])) return fail(HODU_ROCM_INVALID_ARG, "%s: metadata[%zu] out of range", what, i);
+    return HODU_ROCM_OK;
+}
+// `pages` pages of `page_size` tokens are numbered with 32-bit slots
+int check_pages(const char *what, size_t pages, size_t page_size, const char *of) {
+    if (page_size < 1) return fail(HODU_ROCM_INVALID_ARG, "%s: a page holds at least one token", what);
+    if (page_size > kMaxInt || pages > kMaxInt || pages * page_size > kMaxInt)
+        return fail(HODU_ROCM_UNSUPPORTED, "%s: %zu pages of %zu tokens (%s) do not fit 32-bit slots", what, pages, page_size, of);
+    return HODU_ROCM_OK;
+}
+int check_heads(const char *what, size_t batch, size_t tokens, size_t heads, size_t kv_heads) {
+    if (batch > kMaxInt - 1 || tokens > kMaxInt || heads > kMaxInt || kv_heads > kMaxInt)
+        return fail(HODU_ROCM_UNSUPPORTED, "%s: more than 2^31 - 1 sequences, tokens or heads", what);
+    if (kv_heads < 1 || heads < 1 || heads % kv_heads)
+        return fail(HODU_ROCM_INVALID_ARG, "%s: %zu heads do not share %zu key / value heads evenly", what, heads, kv_heads);
+    if (tokens * (heads / kv_heads) > kMaxInt)
+        return fail(HODU_ROCM_UNSUPPORTED, "%s: %zu tokens of %zu heads per key / value head exceed 2^31 - 1 rows", what, tokens, heads / kv_heads);
+    return HODU_ROCM_OK;
+}
+}  // namespace
+
+// [batch, page_size, width, n_free, capacity]
+int parse_paged_plan_metadata(const size_t *md, size_t len, PagedPlanArgs *a) {
+    if (int rc = check_words("paged_plan", md, len, 5)) return rc;
+    if (int rc = check_pages("paged_plan", md[2], md[1], "a table row")) return rc;
+    if (md[3] > kMaxInt || md[4] > kMaxInt)
+        return fail(HODU_ROCM_UNSUPPORTED, "paged_plan: more than 2^31 - 1 free pages or slots");
+    *a = PagedPlanArgs{};
+    a->batch = (long)md[0]; a->page_size = (long)md[1]; a->width = (long)md[2]; a->n_free = (long)md[3]; a->capacity = (long)md[4];
+    return HODU_ROCM_OK;
+}
+
+// [tokens, kv_heads, D, k_token, k_head, v_token, v_head, k_off, v_off, n_pages, page_size, k cache (page, token, head),
+//  v cache (page, token, head), k_cache_off, v_cache_off]
+int parse_paged_store_metadata(const size_t *md, size_t len, PagedStoreArgs *a) {
+    if (int rc = check_words("paged_store", md, len, 19)) return rc;
+    if (int rc = check_pages("paged_store", md[9], md[10], "the cache")) return rc;
+    if (md[0] > kMaxInt || md[1] > kMaxInt || md[2] > kMaxInt || md[1] * md[2] > kMaxInt)
+        return fail(HODU_ROCM_UNSUPPORTED, "paged_store: more than 2^31 - 1 tokens or elements of a token");
+    *a = PagedStoreArgs{};
+    a->tokens = (long)md[0]; a->kv_heads = (long)md[1]; a->d = (long)md[2];
+    a->k_token = (long)md[3]; a->k_head = (long)md[4]; a->v_token = (long)md[5]; a->v_head = (long)md[6];
+    a->k_off = (long)md[7]; a->v_off = (long)md[8];
+    a->n_pages = (long)md[9]; a->page_size = (long)md[10];
+    a->kc.page = (long)md[11]; a->kc.token = (long)md[12]; a->kc.head = (long)md[13];
+    a->vc.page = (long)md[14]; a->vc.token = (long)md[15]; a->vc.head = (long)md[16];
+    a->kc.off = (long)md[17]; a->vc.off = (long)md[18];
+    return HODU_ROCM_OK;
+}
+
+// [batch, q_tokens, k_tokens, heads, kv_heads, D, q_token, q_head, k_token, k_head, v_token, v_head, q_off, k_off, v_off]
+int parse_varlen_metadata(const size_t *md, size_t len, SeqAttentionArgs *a) {
+    if (int rc = check_words("attention_varlen", md, len, 15)) return rc;
+    if (int rc = check_heads("attention_varlen", md[0], md[1], md[3], md[4])) return rc;
+    if (md[2] > kMaxInt) return fail(HODU_ROCM_UNSUPPORTED, "attention_varlen: more than 2^31 - 1 keys");
+    *a = SeqAttentionArgs{};
+    a->batch = (long)md[0]; a->q_tokens = (long)md[1]; a->k_tokens = (long)md[2];
+    a->heads = (long)md[3]; a->kv_heads = (long)md[4]; a->d = (long)md[5];
+    a->q_token = (long)md[6]; a->q_head = (long)md[7];
+    a->kc.token = (long)md[8]; a->kc.head = (long)md[9];
+    a->vc.token = (long)md[10]; a->vc.head = (long)md[11];
+    a->q_off = (long)md[12]; a->kc.off = (long)md[13]; a->vc.off = (long)md[14];
+    return HODU_ROCM_OK;
+}
+
+// [batch, q_tokens, heads, kv_heads, D, n_pages, page_size, width, q_token, q_head, q_off, k cache (page, token, head),
+//  v cache (page, token, head), k_cache_off, v_cache_off]
+int parse_paged_attention_metadata(const size_t *md, size_t len, SeqAttentionArgs *a) {
+    if (int rc = check_words("attention_paged", md, len, 19)) return rc;
+    if (int rc = check_heads("attention_paged", md[0], md[1], md[2], md[3])) return rc;
+    if (int rc = check_pages("attention_paged", md[5], md[6], "the cache")) return rc;
+    if (int rc = check_pages("attention_paged", md[7], md[6], "a table row")) return rc;
+    *a = SeqAttentionArgs{};
+    a->paged = true;
+    a->causal = true;
+    a->batch = (long)md[0]; a->q_tokens = (long)md[1]; a->heads = (long)md[2]; a->kv_heads = (long)md[3]; a->d = (long)md[4];
+    a->n_pages = (long)md[5]; a->page_size = (long)md[6]; a->width = (long)md[7];
+    a->q_token = (long)md[8]; a->q_head = (long)md[9]; a->q_off = (long)md[10];
+    a->kc.page = (long)md[11]; a->kc.token = (long)md[12]; a->kc.head = (long)md[13];
+    a->vc.page = (long)md[14]; a->vc.token = (long)md[15]; a->vc.head = (long)md[16];
+    a->kc.off = (long)md[17]; a->vc.off = (long)md[18];
+    return HODU_ROCM_OK;
+}
+
 }  // namespace hodu

@@ -114,6 +114,10 @@ def declare_compute(lib: ctypes.CDLL):
     lib.hodu_rocm_softmax_masked.argtypes = [vp, ci, vp, vp, szp, sz, ci, vp, ci, szp, sz]
     lib.hodu_rocm_attention.argtypes = [vp, ci, vp, vp, vp, vp, szp, sz, vp, ci]
     lib.hodu_rocm_attention_masked.argtypes = [vp, ci, vp, vp, vp, vp, szp, sz, vp, ci, vp, ci, szp, sz]
+    lib.hodu_rocm_paged_plan.argtypes = [vp] * 9 + [szp, sz]
+    lib.hodu_rocm_paged_store.argtypes = [vp, ci, ci] + [vp] * 7 + [szp, sz]
+    lib.hodu_rocm_attention_varlen.argtypes = [vp, ci] + [vp] * 6 + [szp, sz, vp, ci]
+    lib.hodu_rocm_attention_paged.argtypes = [vp, ci, ci] + [vp] * 9 + [szp, sz, vp]
     lib.hodu_rocm_dot_bf16_f8e4m3w_noalloc.argtypes = [vp, vp, vp, vp, szp, sz]
     lib.hodu_rocm_ctx_set_reference_sums.argtypes = [vp, ci]
 
@@ -205,6 +209,56 @@ def product_spans(op: str, md: Sequence[int]):
     return _view_span(ls, lst, lo), _view_span(rs, rst, ro), md[0]
 
 
+# ---- metadata of the paged cache and of packed sequences (include/hodu_rocm_kernels.h); strides and offsets in elements ----
+def paged_plan_md(batch: int, page_size: int, width: int, n_free: int, capacity: int):
+    """hodu_rocm_paged_plan: requests, tokens of a page, columns of the table, pages on the free list, slots to fill"""
+    return (batch, page_size, width, n_free, capacity)
+
+
+def paged_store_md(tokens: int, kv_heads: int, dim: int, n_pages: int, page_size: int, k_strides=None, v_strides=None,
+                   k_cache_strides=None, v_cache_strides=None, k_offset: int = 0, v_offset: int = 0, k_cache_offset: int = 0,
+                   v_cache_offset: int = 0):
+    """hodu_rocm_paged_store: k / v strides (token, head), cache strides (page, token, head); default: contiguous
+    [tokens, kv_heads, dim] and [n_pages, page_size, kv_heads, dim]"""
+    rows, cache = (kv_heads * dim, dim), (page_size * kv_heads * dim, kv_heads * dim, dim)
+    return (tokens, kv_heads, dim, *(k_strides or rows), *(v_strides or rows), k_offset, v_offset, n_pages, page_size,
+            *(k_cache_strides or cache), *(v_cache_strides or cache), k_cache_offset, v_cache_offset)
+
+
+def varlen_md(batch: int, q_tokens: int, k_tokens: int, heads: int, kv_heads: int, dim: int, q_strides=None, k_strides=None,
+              v_strides=None, q_offset: int = 0, k_offset: int = 0, v_offset: int = 0):
+    """hodu_rocm_attention_varlen: strides (token, head); default: contiguous [tokens, heads, dim]"""
+    q, kv = (heads * dim, dim), (kv_heads * dim, dim)
+    return (batch, q_tokens, k_tokens, heads, kv_heads, dim, *(q_strides or q), *(k_strides or kv), *(v_strides or kv), q_offset,
+            k_offset, v_offset)
+
+
+def paged_attention_md(batch: int, q_tokens: int, heads: int, kv_heads: int, dim: int, n_pages: int, page_size: int, width: int,
+                       q_strides=None, k_cache_strides=None, v_cache_strides=None, q_offset: int = 0, k_cache_offset: int = 0,
+                       v_cache_offset: int = 0):
+    """hodu_rocm_attention_paged: q strides (token, head), cache strides (page, token, head); default: contiguous
+    [q_tokens, heads, dim] and [n_pages, page_size, kv_heads, dim]; table [batch, width]"""
+    cache = (page_size * kv_heads * dim, kv_heads * dim, dim)
+    return (batch, q_tokens, heads, kv_heads, dim, n_pages, page_size, width, *(q_strides or (heads * dim, dim)), q_offset,
+            *(k_cache_strides or cache), *(v_cache_strides or cache), k_cache_offset, v_cache_offset)
+
+
+def _span3(d0, d1, d2, s0, s1, offset):
+    """elements a [d0, d1, d2] view with a dense last dim can touch"""
+    return offset + (d0 - 1) * s0 + (d1 - 1) * s1 + d2 if d0 and d1 and d2 else 0
+
+
+def _span4(d0, d1, d2, d3, s0, s1, s2, offset):
+    return offset + (d0 - 1) * s0 + (d1 - 1) * s1 + (d2 - 1) * s2 + d3 if d0 and d1 and d2 and d3 else 0
+
+
+def _within(what, *needs):
+    """refuse a launch that reaches past one of the device buffers; needs: (name, buffer, bytes)"""
+    for name, buf, nbytes in needs:
+        if nbytes > buf.nbytes:
+            raise HoduRocmError(INVALID_ARG, f"{what}: addresses {nbytes} bytes of {name} but the buffer holds {buf.nbytes}")
+
+
 def _md_array(md: Sequence[int]):
     arr = (ctypes.c_size_t * len(md))(*[int(v) for v in md])
     return arr, len(md)
@@ -230,6 +284,22 @@ class DeviceBuffer:
             self.free()
         except Exception:
             pass
+
+
+class DeviceView:
+    """Device memory that somebody else owns (another library's tensor, a part of a DeviceBuffer), as an operand: the
+    calls that take a DeviceBuffer take one of these.  The owner keeps the memory alive and orders its own work on it
+    against the context's stream."""
+    __slots__ = ("ptr", "nbytes")
+
+    def __init__(self, ptr: int, nbytes: int):
+        self.ptr, self.nbytes = ptr, nbytes
+
+    @classmethod
+    def of(cls, tensor) -> "DeviceView":
+        """of a torch tensor: from its first element to the end of its storage"""
+        storage, size = tensor.untyped_storage(), tensor.element_size()
+        return cls(tensor.data_ptr(), storage.nbytes() - tensor.storage_offset() * size)
 
 
 class Context:
@@ -444,6 +514,75 @@ class Context:
             return
         self._check(self.lib.hodu_rocm_attention(self.handle, DTYPE_ID[dt], q.ptr, k.ptr, v.ptr, out.ptr, arr, n,
                                                  sc.ctypes.data, int(bool(causal))))
+
+    def paged_plan(self, cached, added, free_pages, table, lens, offsets, slots, used, md):
+        """hodu_rocm_paged_plan: block tables and slot maps from request lengths; md: paged_plan_md(..).  All operands
+        are i32 device buffers; free_pages and slots may be None where the list or the capacity is empty"""
+        if len(md) == 5:
+            b, _, width, n_free, capacity = md
+            _within("paged_plan", ("cached", cached, 4 * b), ("added", added, 4 * b), ("table", table, 4 * b * width), ("lens", lens, 4 * b),
+                    ("offsets", offsets, 4 * b + 4), ("used", used, 8))
+            for name, buf, n in (("free_pages", free_pages, n_free), ("slots", slots, capacity)):
+                if buf is not None:
+                    _within("paged_plan", (name, buf, 4 * n))
+        arr, n = _md_array(md)
+        self._check(self.lib.hodu_rocm_paged_plan(
+            self.handle, cached.ptr, added.ptr, None if free_pages is None else free_pages.ptr, table.ptr, lens.ptr, offsets.ptr,
+            None if slots is None else slots.ptr, used.ptr, arr, n))
+
+    def paged_store(self, dt: str, k, v, k_cache, v_cache, slots, md, cache_dt: Optional[str] = None, k_scale=None, v_scale=None):
+        """hodu_rocm_paged_store: new keys and values into their slots of the cache; md: paged_store_md(..); cache_dt: dt
+        (default) or "f8e4m3" with k_scale / v_scale, f32 device buffers of one scale per kv head"""
+        cache_dt = cache_dt or dt
+        if len(md) == 19:
+            t, h, d, kt, kh, vt, vh, ko, vo, pages, page, kcp, kct, kch, vcp, vct, vch, kco, vco = md
+            es, ces = DTYPE_SIZE[dt], DTYPE_SIZE[cache_dt]
+            _within("paged_store", ("k", k, _span3(t, h, d, kt, kh, ko) * es), ("v", v, _span3(t, h, d, vt, vh, vo) * es),
+                    ("k_cache", k_cache, _span4(pages, page, h, d, kcp, kct, kch, kco) * ces),
+                    ("v_cache", v_cache, _span4(pages, page, h, d, vcp, vct, vch, vco) * ces), ("slots", slots, 4 * t))
+            for name, buf in (("k_scale", k_scale), ("v_scale", v_scale)):
+                if buf is not None:
+                    _within("paged_store", (name, buf, 4 * h))
+        arr, n = _md_array(md)
+        self._check(self.lib.hodu_rocm_paged_store(
+            self.handle, DTYPE_ID[dt], DTYPE_ID[cache_dt], k.ptr, v.ptr, k_cache.ptr, v_cache.ptr, slots.ptr,
+            None if k_scale is None else k_scale.ptr, None if v_scale is None else v_scale.ptr, arr, n))
+
+    def attention_varlen(self, dt: str, q, k, v, out, q_offsets, k_offsets, md, scale, causal: bool = False):
+        """hodu_rocm_attention_varlen: attention over packed sequences; md: varlen_md(..); q_offsets, k_offsets: i32 device
+        buffers of batch + 1; scale: 1-element array in dt's storage"""
+        if len(md) == 15:
+            b, tq, tk, hq, hk, d, qt, qh, kt, kh, vt, vh, qo, ko, vo = md
+            es = DTYPE_SIZE[dt]
+            _within("attention_varlen", ("q", q, _span3(tq, hq, d, qt, qh, qo) * es), ("k", k, _span3(tk, hk, d, kt, kh, ko) * es),
+                    ("v", v, _span3(tk, hk, d, vt, vh, vo) * es), ("out", out, tq * hq * d * es), ("q_offsets", q_offsets, 4 * b + 4),
+                    ("k_offsets", k_offsets, 4 * b + 4))
+        arr, n = _md_array(md)
+        sc = np.ascontiguousarray(scale).reshape(1)
+        self._check(self.lib.hodu_rocm_attention_varlen(self.handle, DTYPE_ID[dt], q.ptr, k.ptr, v.ptr, out.ptr, q_offsets.ptr,
+                                                        k_offsets.ptr, arr, n, sc.ctypes.data, int(bool(causal))))
+
+    def attention_paged(self, dt: str, q, k_cache, v_cache, out, q_offsets, table, lens, md, scale, cache_dt: Optional[str] = None,
+                        k_scale=None, v_scale=None):
+        """hodu_rocm_attention_paged: attention of each request's last tokens over its pages of the cache; md:
+        paged_attention_md(..); table [batch, width], lens [batch], q_offsets [batch + 1]: i32 device buffers; cache_dt and
+        the scales as for paged_store"""
+        cache_dt = cache_dt or dt
+        if len(md) == 19:
+            b, tq, hq, hk, d, pages, page, width, qt, qh, qo, kcp, kct, kch, vcp, vct, vch, kco, vco = md
+            es, ces = DTYPE_SIZE[dt], DTYPE_SIZE[cache_dt]
+            _within("attention_paged", ("q", q, _span3(tq, hq, d, qt, qh, qo) * es),
+                    ("k_cache", k_cache, _span4(pages, page, hk, d, kcp, kct, kch, kco) * ces),
+                    ("v_cache", v_cache, _span4(pages, page, hk, d, vcp, vct, vch, vco) * ces), ("out", out, tq * hq * d * es),
+                    ("q_offsets", q_offsets, 4 * b + 4), ("table", table, 4 * b * width), ("lens", lens, 4 * b))
+            for name, buf in (("k_scale", k_scale), ("v_scale", v_scale)):
+                if buf is not None:
+                    _within("attention_paged", (name, buf, 4 * hk))
+        arr, n = _md_array(md)
+        sc = np.ascontiguousarray(scale).reshape(1)
+        self._check(self.lib.hodu_rocm_attention_paged(
+            self.handle, DTYPE_ID[dt], DTYPE_ID[cache_dt], q.ptr, k_cache.ptr, v_cache.ptr, out.ptr, q_offsets.ptr, table.ptr, lens.ptr,
+            None if k_scale is None else k_scale.ptr, None if v_scale is None else v_scale.ptr, arr, n, sc.ctypes.data))
 
     def time_product(self, op: str, name: str, lhs: DeviceBuffer, rhs_list, out: DeviceBuffer, md, iters: int,
                      graph: bool = False, steps=None) -> float:

@@ -279,6 +279,72 @@ int hodu_rocm_attention_masked(hodu_rocm_ctx *ctx, int dtype, const void *q, con
                                const size_t *metadata, size_t metadata_len, const void *scale, int causal,
                                const void *mask, int mask_dtype, const size_t *mask_layout, size_t mask_layout_len);
 
+/* ---- the attention side of a serving loop: a paged key / value cache and packed sequences -------------------- *
+ * No counterpart in the reference, whose attention takes one dense batch of equal lengths; these are what a caller of
+ * hodu_rocm_attention needs once requests differ in length, share key / value heads and grow token by token.
+ *
+ * The cache of keys (and one like it of values) is n_pages pages of page_size tokens of kv_heads heads of D elements,
+ * in any order of pages, tokens and heads (element strides; the D elements dense).  Request r's token t lives in page
+ * table[r][t / page_size], at t % page_size.  A slot is page * page_size + (token of the page), as a 32-bit number.
+ * All int arrays are DEVICE memory, 4-byte aligned; metadata is host memory, as everywhere in this header.
+ * A loop's step is: paged_plan, the model's projections, paged_store, attention_paged -- in stream order, nothing of
+ * it read back on the host, every call fit for capture into a graph. */
+
+/* Block tables and slot maps from request lengths.  For each of `batch` requests with cached[r] tokens in the cache and
+ * added[r] new ones: the pages it lacks are taken from free_pages[0 .. n_free), in the order of the requests, and
+ * entered into table[r][held ..] (held = ceil(cached / page_size); the row's other entries stay as they are); lens[r] =
+ * cached + added; offsets[0 .. batch] = the new tokens' running count, which is where each request's rows begin among
+ * the packed new tokens; slots[t] = where new token t is to be stored, -1 from the last token up to `capacity`;
+ * used[0] = pages taken (always the first of the list), used[1] = requests refused.  A request is refused -- it adds
+ * no token, takes no page, and lens[r] is what was cached (0 if that is negative) -- when a length is negative, when it outgrows `width`
+ * pages, when the list holds too few pages for it, or when its tokens pass `capacity`; the list and the capacity are
+ * dealt out in order, so once one of them ran out every later request that needs it is refused too.
+ * metadata: [batch, page_size, width, n_free, capacity]; at most 16384 requests.  Outputs and inputs must not overlap. */
+int hodu_rocm_paged_plan(hodu_rocm_ctx *ctx, const int *cached, const int *added, const int *free_pages, int *table, int *lens,
+                         int *offsets, int *slots, int *used, const size_t *metadata, size_t metadata_len);
+
+/* New keys and values into their slots: cache[slots[t]][h] = k[t][h].  dtype: bf16 or f16, of k and v; cache_dtype: the
+ * same, or f8e4m3 (OCP E4M3FN) with a scale per head in k_scale / v_scale (device f32, kv_heads each; null otherwise):
+ * the cache then holds k / scale, divided in f32, rounded to nearest even and saturated at 448 (NaN stays NaN).  A slot
+ * that is negative or beyond the cache is skipped.  A slot that two tokens name holds pieces of either.
+ * metadata: [tokens, kv_heads, D, k_token, k_head, v_token, v_head, k_off, v_off, n_pages, page_size, k cache strides
+ * (page, token, head), v cache strides (page, token, head), k_cache_off, v_cache_off]; D, strides and offsets multiples
+ * of 8 elements, bases of 16 bytes. */
+int hodu_rocm_paged_store(hodu_rocm_ctx *ctx, int dtype, int cache_dtype, const void *k, const void *v, void *k_cache,
+                          void *v_cache, const int *slots, const float *k_scale, const float *v_scale,
+                          const size_t *metadata, size_t metadata_len);
+
+/* Attention over packed sequences of different lengths: q [q_tokens, heads, D], k and v [k_tokens, kv_heads, D], the
+ * sequences one after the other: sequence b is rows q_offsets[b] .. q_offsets[b + 1] of q and rows k_offsets[b] .. of k
+ * and v (device, batch + 1 each; the same array for self-attention).  Query head h reads key / value head
+ * h / (heads / kv_heads).  causal != 0: row i of n rows over m keys attends keys 0 .. i + m - n (the last row all of
+ * them).  A row that attends no key is zero; rows of out behind the last sequence are left as they were; offsets are
+ * clamped to the packed lengths.  Scores, softmax and the sums over keys are f32; the probabilities are rounded to
+ * `dtype` as the second product's operand and the result once.  out: contiguous [q_tokens, heads, D].
+ * dtype: bf16 or f16; D = 64 or 128; the D elements dense, strides and offsets multiples of 8 elements, bases of 16
+ * bytes; scale: the scalar in `dtype`, positive and finite.  HODU_ROCM_UNSUPPORTED otherwise.
+ * metadata: [batch, q_tokens, k_tokens, heads, kv_heads, D, q_token, q_head, k_token, k_head, v_token, v_head, q_off,
+ * k_off, v_off] (element strides between tokens and heads). */
+int hodu_rocm_attention_varlen(hodu_rocm_ctx *ctx, int dtype, const void *q, const void *k, const void *v, void *out,
+                               const int *q_offsets, const int *k_offsets, const size_t *metadata, size_t metadata_len,
+                               const void *scale, int causal);
+
+/* Attention of new tokens over the paged cache, a chunk of a prompt or a single token alike: request r's rows
+ * q_offsets[r] .. q_offsets[r + 1] of q are the LAST ones of its lens[r] tokens, whose keys and values -- the new
+ * tokens' among them -- are in the cache; row i of n attends keys 0 .. lens[r] - n + i.  Otherwise as
+ * hodu_rocm_attention_varlen.  cache_dtype and the scales as for hodu_rocm_paged_store: an f8e4m3 cache is widened
+ * exactly and counts as value * scale (scales positive and finite).  Slots beyond lens[r] are never read: they may hold
+ * anything.  Table entries of tokens below lens[r] have to be pages of the cache; an entry that is not is clamped to
+ * one, so that nothing outside the cache is read.  Offsets, strides and bases of an f8e4m3 cache: multiples of 16.
+ * metadata: [batch, q_tokens, heads, kv_heads, D, n_pages, page_size, width, q_token, q_head, q_off, k cache strides
+ * (page, token, head), v cache strides (page, token, head), k_cache_off, v_cache_off]; table is [batch, width].
+ * Calls with few rows over long contexts cut the keys into ranges and keep partial results in the context's workspace,
+ * which may have to grow: run such a call once before capturing it. */
+int hodu_rocm_attention_paged(hodu_rocm_ctx *ctx, int dtype, int cache_dtype, const void *q, const void *k_cache,
+                              const void *v_cache, void *out, const int *q_offsets, const int *table, const int *lens,
+                              const float *k_scale, const float *v_scale, const size_t *metadata, size_t metadata_len,
+                              const void *scale);
+
 #ifdef __cplusplus
 }
 #endif

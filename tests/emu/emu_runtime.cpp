@@ -89,6 +89,16 @@ NOT_IN_THIS_LIBRARY(launch_gemv_rows)
 int launch_attention(hodu_rocm_ctx *, int, const void *, const void *, const void *, void *, const AttentionArgs &, const AttentionMask *) {
     return HODU_ROCM_UNSUPPORTED;
 }
+int launch_seq_attention(hodu_rocm_ctx *, int, int, const void *, const void *, const void *, void *, const SeqAttentionArgs &) {
+    return HODU_ROCM_UNSUPPORTED;
+}
+int launch_paged_plan(hodu_rocm_ctx *, const int *, const int *, const int *, int *, int *, int *, int *, int *, const PagedPlanArgs &) {
+    return HODU_ROCM_UNSUPPORTED;
+}
+int launch_paged_store(hodu_rocm_ctx *, int, int, const void *, const void *, void *, void *, const int *, const float *, const float *,
+                       const PagedStoreArgs &) {
+    return HODU_ROCM_UNSUPPORTED;
+}
 }  // namespace hodu
 
 extern "C" {

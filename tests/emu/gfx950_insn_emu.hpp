@@ -226,6 +226,16 @@ inline vbf16x2 cvt_pk_bf16_fp8(unsigned word, float scale, bool hi) {
     return __builtin_bit_cast(vbf16x2, both);
 }
 
+// the same into f16: every f8e4m3 value is an f16 value (its subnormals are normal there)
+typedef _Float16 vf16x2 __attribute__((ext_vector_type(2)));
+inline vf16x2 cvt_pk_f16_fp8(unsigned word, float scale, bool hi) {
+    if (scale != 1.0f) (void)no_such_instruction("cvt_scalef32_pk_f16_fp8 with a scale");
+    const unsigned half = hi ? word >> 16 : word & 0xFFFFu;
+    return vf16x2{(_Float16)f8_decode<4, 3>(half & 0xFF), (_Float16)f8_decode<4, 3>(half >> 8)};
+}
+// ds_bpermute_b32: a lane receives what the lane numbered by its address / 4 (modulo 64) holds
+inline int ds_bpermute(int addr, int v) { return (int)slot_u32(wave_values((unsigned)v), ((unsigned)addr >> 2) & 63u); }
+
 // v_perm_b32: result byte i is byte sel[i] of the eight bytes {s1 (0..3), s0 (4..7)}; selectors above 7 (sign fills and
 // constants) are not used by these kernels
 inline unsigned perm_b32(unsigned s0, unsigned s1, unsigned sel) {
@@ -278,6 +288,8 @@ struct Any {
 #define __builtin_amdgcn_ds_read_tr16_b64_v4i16(p) (emu::ds_read_tr<2, short __attribute__((ext_vector_type(4)))>((const void *)(p)))
 #define __builtin_amdgcn_ds_read_tr8_b64_v2i32(p) (emu::ds_read_tr<1, int __attribute__((ext_vector_type(2)))>((const void *)(p)))
 #define __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, hi) emu::cvt_pk_bf16_fp8(w, scale, hi)
+#define __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, hi) emu::cvt_pk_f16_fp8(w, scale, hi)
+#define __builtin_amdgcn_ds_bpermute(addr, v) emu::ds_bpermute(addr, v)
 #define __builtin_amdgcn_global_load_lds(g, l, size, off, aux) \
     (EMU_M0_WRITTEN = true, emu::dma16((const char *)(g), (unsigned)(uintptr_t)(l)))
 #define EMU_MFMA(ROWS, WIDEN, a, b, c) \

@@ -36,7 +36,7 @@ LIB = os.path.join(OUT, "libhodu_emu.so")
 MFMA_SOURCES = [os.path.join(CSRC, f) for f in ("gemm_mfma.hip", "gemm_mfma_bf16.hip", "gemm_mfma_mi16_bf16.hip", "gemm_mfma_w8a16.hip",
                                                 "gemm_mfma_f16.hip", "gemm_mfma_mi16_f16.hip", "gemm_mfma_f32.hip", "gemm_mfma_i8.hip",
                                                 "gemm_mfma_i8_out.hip", "gemm_mfma_u8_out.hip", "gemm_mfma_f8.hip", "skinny.hip",
-                                                "gemv.hip", "gemv_rows.hip", "small_f32.hip", "gemm_f64.hip", "attention.hip", "runtime.cpp")] + \
+                                                "gemv.hip", "gemv_rows.hip", "small_f32.hip", "gemm_f64.hip", "attention.hip", "attention_seq.hip", "paged.hip", "runtime.cpp")] + \
                [os.path.join(ROOT, "hodu_amd", "csrc_debug", "timing.cpp")]
 MFMA_LIB = os.path.join(OUT, "libhodu_emu_mfma.so")
 
