@@ -329,6 +329,407 @@ __global__ __launch_bounds__(R16_NT) void seq_attention_r16_kernel(const uint16_
     else *reinterpret_cast<u32x2_t *>(dst) = u32x2_t{out[0], out[1]};
 }
 
+// ---- tiles of 128, 192 or 256 rows, one wavefront per SIMD ---------------------------------------------------------------
+// The matrix cores bound a long prompt: 4 D flops per (row, key) pair against 2 D / rows bytes.  Four wavefronts own 16 RT
+// rows each (RT = 2, 3 or 4 tiles of 16) and walk all keys of the tile, 64 to a stage of the LDS ring, 32 to a step, with the layouts of the
+// kernel above.  A fragment of K or V read from LDS feeds RT matrix instructions, which is what keeps LDS from being the bound
+// (128 bytes a cycle: a fragment per 2 RT cycles of each SIMD; the instruction takes 16).
+//
+// A wavefront issues in order, an instruction every 4 cycles, and a matrix instruction runs for 16: the exponentials have
+// to stand BETWEEN the matrix instructions.  So a step holds three independent pieces of work -- scores of step i + 1,
+// exponentials of step i, P V of step i - 1 -- written out as one sequence of chunks, a matrix instruction and
+// a share of the vector work and LDS reads in each, which the compiler may not reorder across (sched_barrier, and the empty
+// statements that pin a chunk's results to it).
+//
+// The exponent reference of a row is an integer E >= c max - SLACK, c = scale log2 e: p = 2^(c s - E) <= 2^SLACK (f32 and bf16 reach to 2^127, f16 to 2^16).  It moves only when a
+// score exceeds it by 2^SLACK, which the lanes find out without talking to each other (any lane's own maximum); then the row's lanes
+// agree on the new one and O, the row sum and the P not yet multiplied are rescaled -- by a power of two, exactly.
+// Row tiles per wavefront: 3 at head dim 128 (O, q, two steps' scores and P are 84 registers a tile; with 4 the allocator runs out),
+// 4 at 64.
+template <int D> constexpr int W_TILES = D == 128 ? 3 : 4;
+constexpr int W_NT = 256, W_BK = 64, W_RING = 4, W_WINDOW = 2048;  // (the ring: stages of K and of V)
+template <int D, bool F8, bool PAGED> struct WGeom {
+    typedef R16Geom<D, F8> R;
+    static constexpr int ROW = R::ROW, CPR = R::CPR, KPI = R::KPI;   // bytes and chunks of a row, keys of an LDS-DMA instruction
+    static constexpr int BLOCK = W_BK * ROW, NI = W_BK / KPI / 4;    // instructions per block and wavefront
+    static constexpr int KS = R::KS, DT = R::DT;
+    static constexpr int V_AT = W_RING * BLOCK, TABLE_AT = 2 * V_AT;
+    static constexpr int LDS = TABLE_AT + (PAGED ? W_WINDOW * 4 : 0);
+};
+
+template <int CK, int D, bool PAGED, bool F8, int RT>
+__global__ __launch_bounds__(W_NT, 1) void seq_attention_wide_kernel(const uint16_t *__restrict__ Q, const char *__restrict__ K,
+                                                                     const char *__restrict__ V, uint16_t *__restrict__ O, DevSeq a) {
+    typedef WGeom<D, F8, PAGED> G;
+    typedef R16Geom<D, F8> R;
+    typedef Compute<CK> Cmp;
+    typedef typename Cmp::acc_t acc_t;
+    constexpr int KS = G::KS, DT = G::DT, BM = 64 * RT;
+    constexpr bool F16 = CK == mfma::CK_F16;
+    HODU_DYNAMIC_LDS(smem);
+    const unsigned lds0 = (unsigned)(uintptr_t)smem;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 15, g = lane >> 4;
+    const int kvh = blockIdx.x % a.kv_heads;
+    int b, row0, q0, n, k0, m;
+    if (!find_tile<BM>(a, blockIdx.x / a.kv_heads, b, row0, q0, n)) return;
+    find_keys<PAGED>(a, b, k0, m);
+
+    const int rows = n * a.group;
+    // the lane's rows, one per tile; rows past the sequence's last repeat it and are not stored
+    int open[RT];
+    u32x4_t qf[RT][KS];
+    const int wrow0 = row0 + wave * 16 * RT;
+#pragma unroll
+    for (int x = 0; x < RT; x++) {
+        const int row = wrow0 + 16 * x + r, rr = row < rows ? row : rows - 1;
+        const int tok = quot(rr, a.by_group), head = kvh * a.group + rr - tok * a.group;
+        open[x] = a.causal ? tok + m - n + 1 : m;  // keys the row attends, <= 0: none
+        const uint16_t *q = Q + (q0 + tok) * a.q_token + head * a.q_head;
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) qf[x][ks] = *reinterpret_cast<const u32x4_t *>(q + 32 * ks + 8 * g);
+    }
+    const float c = a.scale_log2e * (F8 ? a.k_scale[kvh] : 1.f);
+    auto last_row = [&](int i) { return i < rows ? i : rows - 1; };
+    const int keys_any = a.causal ? quot(last_row(row0 + BM - 1), a.by_group) + m - n + 1 : m;  // keys the tile needs
+    const int keys = keys_any > 0 ? keys_any : 0;
+    const int wave_keys = a.causal ? quot(last_row(wrow0 + 16 * RT - 1), a.by_group) + m - n + 1 : m;  // ... the wavefront needs
+    const int all_open = a.causal ? quot(last_row(wrow0), a.by_group) + m - n + 1 : m;  // keys below this are open to all its rows
+    const int stages = (keys + W_BK - 1) / W_BK;
+    const int steps = wave_keys > 0 && wrow0 < rows ? (wave_keys + 31) / 32 : 0;  // of 32 keys, that the wavefront needs
+
+    // ---- memory -> LDS: instruction i of a block fills 1 KB, KPI keys; a wavefront issues NI of them for K and for V ----
+    const char *kbase = K + kvh * a.kc.head, *vbase = V + kvh * a.vc.head;
+    int *window = reinterpret_cast<int *>(smem + G::TABLE_AT);
+    int window0 = 0;  // first table column in the window
+    [[maybe_unused]] auto fill_window = [&](int from) __attribute__((always_inline)) {
+        const int cols = quot(keys - 1, a.page) + 1;
+        for (int i = tid; i < W_WINDOW && from + i < cols; i += W_NT) {
+            const int pg = a.table[(long)b * a.width + from + i];
+            window[i] = pg < 0 ? 0 : pg < a.n_pages ? pg : a.n_pages - 1;
+        }
+        window0 = from;
+    };
+    auto issue = [&](int stage, bool is_v) __attribute__((always_inline)) {
+        const int at = (is_v ? G::V_AT : 0) + (stage & (W_RING - 1)) * G::BLOCK;
+#pragma unroll
+        for (int p = 0; p < G::NI; p++) {
+            const int i = wave * G::NI + p, kk = i * G::KPI + lane / G::CPR;
+            int key = stage * W_BK + kk;
+            key = key < keys ? key : keys - 1;  // behind the last key: that one again, masked below
+            const PagedSide &side = is_v ? a.vc : a.kc;
+            long off;
+            if constexpr (PAGED) {
+                const int col = quot(key, a.page);
+                off = window[col - window0] * side.page + (key - col * a.page.d) * side.token;
+            } else {
+                off = (k0 + key) * side.token;
+            }
+            const int chunk = (lane % G::CPR) ^ (is_v ? R::vswz(kk & 31) : R::kswz(kk & 31));
+            mfma::dma16_raw((is_v ? vbase : kbase) + off + (chunk << 4), __builtin_amdgcn_readfirstlane(lds0 + at + i * 1024));
+        }
+    };
+
+    acc_t o[RT][DT];
+    float e_ref[RT], l_run[RT], top[RT];  // exponent reference, the lane's share of the row sum, the lane's largest new score
+#pragma unroll
+    for (int x = 0; x < RT; x++) {
+#pragma unroll
+        for (int j = 0; j < DT; j++) o[x][j] = acc_t{0.f, 0.f, 0.f, 0.f};
+        e_ref[x] = -1e30f;  // no key yet
+        l_run[x] = 0.f;
+    }
+
+    // fragments.  K fragment q = 2 ks + t: 16 keys of tile t, 32 of the head dim (8-bit: raw bytes).  V fragment j: 32 keys, 16 of
+    // the head dim, through VR transpose reads
+    constexpr int KF = 2 * KS, VR = F8 ? 1 : 2;
+    typedef typename std::conditional<F8, u32x2_t, u32x4_t>::type raw_t;
+    raw_t kf[KF];
+    u32x2_t vf[DT * VR];
+    int k_at[2];
+#pragma unroll
+    for (int t = 0; t < 2; t++) {
+        const int key = 8 * (r >> 2) + 4 * t + (r & 3);
+        k_at[t] = key * G::ROW + (((F8 ? g >> 1 : g) ^ R::kswz(key)) << 4) + (F8 ? (g & 1) * 8 : 0);
+    }
+    const int v_key = 8 * g + (F8 ? r >> 1 : r >> 2);
+    const int v_at = G::V_AT + v_key * G::ROW + (((F8 ? 0 : (r >> 1) & 1) ^ R::vswz(v_key)) << 4) + (r & 1) * 8;
+    const int v_at4 = G::V_AT + (v_key + 4) * G::ROW + ((((r >> 1) & 1) ^ R::vswz(v_key + 4)) << 4) + (r & 1) * 8;  // 16-bit: keys + 4
+    auto read_k = [&](int q, int at) __attribute__((always_inline)) {  // (the chunk index is XORed, so a fragment's distance along the head dim is one on the address)
+        const int ks = q >> 1, t = q & 1;
+        if constexpr (F8) kf[q] = lds_get64(smem + at, k_at[t] ^ (ks << 5));
+        else kf[q] = lds_get(smem + at, k_at[t] ^ (ks << 6));
+    };
+    auto k_operand = [&](int q) __attribute__((always_inline)) -> u32x4_t {
+        if constexpr (F8) return widen8<CK>(kf[q]);
+        else return kf[q];
+    };
+    auto read_v = [&](int q, int at) __attribute__((always_inline)) {
+        if constexpr (F8) vf[q] = lds_get_tr<1>(smem + at, v_at ^ (q << 4));
+        else vf[q] = lds_get_tr<2>(smem + at, ((q & 1) ? v_at4 : v_at) ^ ((q >> 1) << 5));
+    };
+    auto v_operand = [&](int j) __attribute__((always_inline)) -> u32x4_t {
+        if constexpr (F8) return widen8<CK>(vf[j]);
+        else return u32x4_t{vf[2 * j].x, vf[2 * j].y, vf[2 * j + 1].x, vf[2 * j + 1].y};
+    };
+    // scores of step i beyond what a row attends; the lane's keys are 8 g + 4 t + e
+    auto mask = [&](acc_t (&sc)[RT][2], int i) __attribute__((always_inline)) {
+#pragma unroll
+        for (int x = 0; x < RT; x++)
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) sc[x][t][e] = i * 32 + 8 * g + 4 * t + e < open[x] ? sc[x][t][e] : -INFINITY;
+    };
+    auto largest = [&](const acc_t (&sc)[RT][2]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int x = 0; x < RT; x++) {
+            top[x] = sc[x][0][0];
+#pragma unroll
+            for (int e = 1; e < 8; e++) top[x] = __builtin_fmaxf(top[x], sc[x][e >> 2][e & 3]);
+        }
+    };
+    // Moves the references of the rows whose new scores exceed them by too much (rare: some lane saw one); pc: the P that is
+    // still to be multiplied
+    constexpr float SLACK = F16 ? 12.f : 64.f;
+    auto move_references = [&](u32x4_t (&pc)[RT]) __attribute__((always_inline)) {
+        mfma::mfma_results_settle();
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int x = 0; x < RT; x++) {
+            float most = __builtin_fmaxf(top[x], __shfl_xor(top[x], 16));
+            most = c * __builtin_fmaxf(most, __shfl_xor(most, 32));
+            const float e_new = most > e_ref[x] + SLACK ? ceilf(most) : e_ref[x];
+            const float f = __builtin_amdgcn_exp2f(e_ref[x] - e_new);
+            e_ref[x] = e_new;
+            l_run[x] *= f;
+#pragma unroll
+            for (int j = 0; j < DT; j++) mfma::scale4_acc(o[x][j], f);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const uint32_t pw = pc[x][i];
+                if constexpr (!F16) pc[x][i] = pack2<CK>(bf16_bits_to_f32((uint16_t)pw) * f, bf16_bits_to_f32((uint16_t)(pw >> 16)) * f);
+                else pc[x][i] = pack2<CK>(f16_bits_to_f32((uint16_t)pw) * f, f16_bits_to_f32((uint16_t)(pw >> 16)) * f);
+            }
+        }
+        mfma::mfma_results_settle();
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    auto some_exceed = [&]() __attribute__((always_inline)) {
+        bool up = false;
+#pragma unroll
+        for (int x = 0; x < RT; x++) up = up || c * top[x] > e_ref[x] + SLACK;
+        return __builtin_amdgcn_ballot_w64(up) != 0;
+    };
+    // element t (of 8 RT) of a step's exponentials
+    float pair;
+    auto exponential = [&](const acc_t (&sc)[RT][2], u32x4_t (&pc)[RT], int t) __attribute__((always_inline)) {
+        const int x = t >> 3, e = t & 7;
+        const float v = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[x][e >> 2][e & 3], c, -e_ref[x]));
+        l_run[x] += v;
+        mfma::pin_vector(l_run[x]);
+        if (e & 1) {
+            pc[x][e >> 1] = pack2<CK>(pair, v);
+            uint32_t w = pc[x][e >> 1];
+            mfma::pin_vector(w);
+            pc[x][e >> 1] = w;
+        } else {
+            pair = v;
+        }
+    };
+    constexpr int NQ = KF * RT, NP = DT * RT, EL = 8 * RT, EVERY = (NQ + NP) / EL;
+    static_assert(EVERY * EL == NQ + NP, "the exponentials spread evenly over the matrix instructions");
+    // Step i of a wavefront whose rows attend all of it and of the next: scores of i + 1 (into sn) and the lane's largest of them,
+    // exponentials of i (sc, into pc), P V of i - 1 (pp).  v_block: where V of step i - 1 lies, k_block: K of step i + 1, k_next: of step
+    // i + 2.  A fragment is read AHEAD chunks (16 cycles each) before its first use: the first ones of a step in the step before.
+    constexpr int AHEAD = NQ < 10 ? NQ : 10;
+    auto first_fragments = [&](int k_block) __attribute__((always_inline)) {
+#pragma unroll
+        for (int q = 0; q < KF; q++)
+            if (q * RT < AHEAD) read_k(q, k_block);
+    };
+    auto step = [&](const acc_t (&sc)[RT][2], acc_t (&sn)[RT][2], const u32x4_t (&pp)[RT], u32x4_t (&pc)[RT], int v_block, int k_block,
+                    int k_next) __attribute__((always_inline)) {
+        constexpr int FROM = NP / 4, MPC = (EL + NP - FROM - 1) / (NP - FROM);
+        static_assert(FROM >= 2 && AHEAD <= NP, "");
+#pragma unroll
+        for (int t = 0; t < NQ + NP; t++) {
+            const int u = t - NQ;  // of the P V instructions
+            if (t < NQ) {
+                // (The scores' matrix instructions name their registers: the allocator would put the scores where the exponentials
+                // cannot read them, 32 copies a step.)
+                const int q = t / RT, x = t % RT;
+                if (q < 2) mfma::mfma16_first<F16, F8>(k_operand(q), qf[x][q >> 1], sn[x][q & 1]);
+                else mfma::mfma16_next<F16, F8>(k_operand(q), qf[x][q >> 1], sn[x][q & 1]);
+            } else {
+                Cmp::mma(v_operand(u / RT), pp[u % RT], o[u % RT][u / RT]);
+            }
+            if (t % EVERY == 0) exponential(sc, pc, t / EVERY);
+            const int soon = t + AHEAD;  // the instruction whose fragment is read now, if it is the first to use it
+            if (soon < NQ) {
+                if (soon % RT == 0) read_k(soon / RT, k_block);
+            } else if (soon < NQ + NP) {
+                if ((soon - NQ) % RT == 0)
+#pragma unroll
+                    for (int w = 0; w < VR; w++) read_v((soon - NQ) / RT * VR + w, v_block);
+            } else if ((soon - NQ - NP) % RT == 0) {
+                read_k((soon - NQ - NP) / RT, k_next);
+            }
+            if (u == FROM) {
+                // Here the scores become values that anything but a matrix instruction may use: the compiler, which knows nothing
+                // of the wait states behind an instruction it has not chosen, copies them for the loop's exits.  (The last one of
+                // them was issued FROM matrix instructions ago: its 4 passes are over.)
+#pragma unroll
+                for (int x = 0; x < RT; x++) {
+                    mfma::pin_vector(sn[x][0]);
+                    mfma::pin_vector(sn[x][1]);
+                }
+            }
+            if (u >= FROM) {  // the lane's largest new score
+#pragma unroll
+                for (int w = 0; w < MPC; w++) {
+                    const int at = (u - FROM) * MPC + w, x = at >> 3, e = at & 7;
+                    if (at < EL) top[x] = e == 0 ? sn[x][0][0] : __builtin_fmaxf(top[x], sn[x][e >> 2][e & 3]);
+                }
+                const int x = ((u - FROM) * MPC + MPC - 1) >> 3;
+                if (x < RT) mfma::pin_vector(top[x]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    // where K or V of step i lies in its ring
+    auto block_of = [&](int i) __attribute__((always_inline)) { return (i >> 1 & (W_RING - 1)) * G::BLOCK + (i & 1) * 32 * G::ROW; };
+    // the same step one piece after the other with few registers, for what is masked, first or last; sc: scores of step i, replaced by
+    // those of i + 1; pc: P of step i - 1, replaced by that of i
+    auto times_v = [&](int i, const u32x4_t (&pp)[RT]) __attribute__((always_inline)) {
+        const int at = block_of(i);
+#pragma unroll
+        for (int j = 0; j < DT; j++) {
+#pragma unroll
+            for (int q = 0; q < VR; q++) read_v(j * VR + q, at);
+#pragma unroll
+            for (int x = 0; x < RT; x++) Cmp::mma(v_operand(j), pp[x], o[x][j]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    auto slow_step = [&](int i, acc_t (&sc)[RT][2], u32x4_t (&pc)[RT]) __attribute__((always_inline)) {
+        if (i > 0) times_v(i - 1, pc);
+        if (i >= 0)
+#pragma unroll
+            for (int t = 0; t < EL; t++) exponential(sc, pc, t);
+        const int at = block_of(i + 1);
+#pragma unroll
+        for (int q = 0; q < KF; q++) {
+            read_k(q, at);
+#pragma unroll
+            for (int x = 0; x < RT; x++) {
+                if (q < 2) sc[x][q & 1] = acc_t{0.f, 0.f, 0.f, 0.f};
+                Cmp::mma(k_operand(q), qf[x][q >> 1], sc[x][q & 1]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        if ((i + 2) * 32 > all_open) mask(sc, i + 1);  // some row does not attend all of step i + 1
+        largest(sc);
+    };
+
+    if (stages > 0) {
+        if constexpr (PAGED) {
+            fill_window(0);
+            __syncthreads();
+        }
+        // step 0 multiplies a P of zeros by what lies where V of the step before it would: zeros too
+        for (int i = tid; i < 32 * G::ROW / 16; i += W_NT)
+            *reinterpret_cast<u32x4_t *>(smem + G::V_AT + (W_RING - 1) * G::BLOCK + 32 * G::ROW + i * 16) = u32x4_t{0, 0, 0, 0};
+        issue(0, false);
+        if (stages > 1) issue(1, false);
+        issue(0, true);
+        if (stages > 2) issue(2, false);
+        if (stages > 1) issue(1, true);
+        __builtin_amdgcn_s_waitcnt(mfma::waitcnt_vm_lgkm0(0));
+        // (pinned, so that the compiler knows on every path into the loop that these loads have returned)
+#pragma unroll
+        for (int x = 0; x < RT; x++)
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) mfma::pin_accumulation(qf[x][ks]);
+        __syncthreads();
+        int st = 0;
+        auto begin_stage = [&]() __attribute__((always_inline)) {
+            // K of stage st + 1 and V of stage st have landed (what was issued at the last stage may be in flight), everybody's;
+            // and everybody is done with what this stage's loads overwrite
+            if (st > 0 && st + 2 < stages) __builtin_amdgcn_s_waitcnt(mfma::waitcnt_vm_lgkm0(2 * G::NI));
+            else __builtin_amdgcn_s_waitcnt(mfma::waitcnt_vm_lgkm0(0));
+            __syncthreads();
+            if constexpr (PAGED) {
+                // the table columns of the keys that are to be loaded: V of stage st + 2 (the least) .. K of stage st + 3
+                const int hi = (st + 4) * W_BK - 1 < keys ? (st + 4) * W_BK - 1 : keys - 1;
+                if (st + 2 < stages && quot(hi, a.page) - window0 >= W_WINDOW) {
+                    fill_window(quot((st + 2) * W_BK, a.page));
+                    __syncthreads();
+                }
+            }
+            if (st + 3 < stages) issue(st + 3, false);
+            if (st + 2 < stages) issue(st + 2, true);
+        };
+        // The stages whose scores are all open run in a loop that holds nothing but the two steps: a rarely taken block that
+        // touches O or P and joins the loop again makes the allocator spill inside it.  Whatever else there is -- an edge, a
+        // reference to move -- leaves the loop, takes slow steps, and comes back.
+        acc_t sc[RT][2];
+        u32x4_t pc[RT];
+#pragma unroll
+        for (int x = 0; x < RT; x++) pc[x] = u32x4_t{0, 0, 0, 0};
+        slow_step(-1, sc, pc);
+        if (some_exceed()) move_references(pc);
+        int i = 0;  // the step in front of us; i = 2 st + 1: in the middle of a stage
+        while (st < stages) {
+            if (!(i & 1) && (2 * st + 3) * 32 <= all_open) {
+                acc_t sn[RT][2];     // scores of the odd steps, those of the even ones in sc
+                u32x4_t pn[RT];      // P of the even steps, that of the odd ones in pc
+                first_fragments(block_of(2 * st + 1));
+                bool half = false;
+                do {
+                    begin_stage();
+                    step(sc, sn, pc, pn, block_of(2 * st - 1), block_of(2 * st + 1), block_of(2 * st + 2));
+                    if (some_exceed()) { half = true; break; }
+                    step(sn, sc, pn, pc, block_of(2 * st), block_of(2 * st + 2), block_of(2 * st + 3));
+                    st++;
+                } while (!some_exceed() && (2 * st + 3) * 32 <= all_open);
+                i = 2 * st + (half ? 1 : 0);
+                if (half) {
+#pragma unroll
+                    for (int x = 0; x < RT; x++) {
+                        sc[x][0] = sn[x][0];
+                        sc[x][1] = sn[x][1];
+                        pc[x] = pn[x];
+                    }
+                }
+            } else {
+                if (!(i & 1)) begin_stage();
+                if (i <= steps) slow_step(i, sc, pc);
+                i++;
+                if (!(i & 1)) st++;
+            }
+            if (i <= steps && some_exceed()) move_references(pc);
+        }
+        if (steps == 2 * stages) times_v(steps - 1, pc);  // P V of the last step
+    }
+
+    // ---- O / l, one rounding: lane (r, g) holds row r of each tile, head-dim columns 16 j + 4 g + e ----
+#pragma unroll
+    for (int x = 0; x < RT; x++) {
+        const int row = wrow0 + 16 * x + r;
+        float l = l_run[x];
+        l += __shfl_xor(l, 16);
+        l += __shfl_xor(l, 32);
+        const float inv = l == 0.f ? 0.f : (F8 ? a.v_scale[kvh] : 1.f) / l;  // a row without keys is zero
+        if (row >= rows) continue;
+        const int tok = quot(row, a.by_group), head = kvh * a.group + row - tok * a.group;
+        uint16_t *dst = O + ((long)(q0 + tok) * a.heads + head) * D;
+#pragma unroll
+        for (int j = 0; j < DT; j++)
+            *reinterpret_cast<u32x2_t *>(dst + 16 * j + 4 * g) =
+                u32x2_t{pack2<CK>(o[x][j][0] * inv, o[x][j][1] * inv), pack2<CK>(o[x][j][2] * inv, o[x][j][3] * inv)};
+    }
+}
+
 }  // namespace
 
 int launch_seq_attention(hodu_rocm_ctx *ctx, int dtype, int cache_dtype, const void *q, const void *k, const void *v, void *out,
@@ -361,20 +762,32 @@ int launch_seq_attention(hodu_rocm_ctx *ctx, int dtype, int cache_dtype, const v
     a.causal = g.causal ? 1 : 0;
     const uint16_t *qp = (const uint16_t *)q + g.q_off;
     const char *kp = (const char *)k + g.kc.off * es, *vp = (const char *)v + g.vc.off * es;
-    const long tiles = (g.q_tokens < g.batch ? g.q_tokens : g.batch) + g.q_tokens * a.group / R16;
-    const long blocks = tiles * g.kv_heads;
-    if (blocks > 0x7FFFFFFFL) return HODU_ROCM_UNSUPPORTED;
-    auto launch = [&](auto kernel, int lds, const char *name) -> int {
+    // rows of a sequence and key / value head, on average
+    const long sequences = g.q_tokens < g.batch ? g.q_tokens : g.batch, avg_rows = g.q_tokens * a.group / sequences;
+    auto launch = [&](auto kernel, int rows, int nt, int lds, const char *name) -> int {
+        const long blocks = (sequences + g.q_tokens * a.group / rows) * g.kv_heads;
+        if (blocks > 0x7FFFFFFFL) return HODU_ROCM_UNSUPPORTED;
         if (int rc = ensure_dynamic_lds(ctx, reinterpret_cast<const void *>(kernel), lds)) return rc;
         ctx->last_kernel = name;
-        hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(R16_NT), lds, ctx->stream, qp, kp, vp, (uint16_t *)out, a);
+        hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(nt), lds, ctx->stream, qp, kp, vp, (uint16_t *)out, a);
         return HODU_ROCM_OK;
     };
-    auto by_type = [&](auto ck, auto d) -> int {
+    auto by_form = [&](auto ck, auto d, auto paged, auto f8_) -> int {
         constexpr int CK = decltype(ck)::value, D = decltype(d)::value;
-        if (!g.paged) return launch(seq_attention_r16_kernel<CK, D, false, false>, R16Geom<D, false>::LDS, "attention_varlen_r16");
-        if (f8) return launch(seq_attention_r16_kernel<CK, D, true, true>, R16Geom<D, true>::LDS, "attention_paged_r16_f8");
-        return launch(seq_attention_r16_kernel<CK, D, true, false>, R16Geom<D, false>::LDS, "attention_paged_r16");
+        constexpr bool PAGED = decltype(paged)::value, F8 = decltype(f8_)::value;
+        const int pin = ctx->force_tile;  // testing hook: 50 tiles of 16 rows, 51 of 128, 52 of 192 or 256
+        if (pin == 52 || (pin < 50 && avg_rows >= 192))
+            return launch(seq_attention_wide_kernel<CK, D, PAGED, F8, W_TILES<D>>, 64 * W_TILES<D>, W_NT, WGeom<D, F8, PAGED>::LDS,
+                          !PAGED ? "attention_varlen_wide" : F8 ? "attention_paged_wide_f8" : "attention_paged_wide");
+        if (pin == 51 || (pin < 50 && avg_rows >= 48))
+            return launch(seq_attention_wide_kernel<CK, D, PAGED, F8, 2>, 128, W_NT, WGeom<D, F8, PAGED>::LDS,
+                          !PAGED ? "attention_varlen_wide128" : F8 ? "attention_paged_wide128_f8" : "attention_paged_wide128");
+        return launch(seq_attention_r16_kernel<CK, D, PAGED, F8>, R16, R16_NT, R16Geom<D, F8>::LDS,
+                      !PAGED ? "attention_varlen_r16" : F8 ? "attention_paged_r16_f8" : "attention_paged_r16");
+    };
+    auto by_type = [&](auto ck, auto d) -> int {
+        if (!g.paged) return by_form(ck, d, std::false_type(), std::false_type());
+        return f8 ? by_form(ck, d, std::true_type(), std::true_type()) : by_form(ck, d, std::true_type(), std::false_type());
     };
     typedef std::integral_constant<int, 64> d64;
     typedef std::integral_constant<int, 128> d128;

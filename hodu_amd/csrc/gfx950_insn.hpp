@@ -27,6 +27,37 @@ __device__ __forceinline__ void mfma16x16x32_f16(const u32x4_t &a, const u32x4_t
     asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
 }
 
+// v_mfma_f32_16x16x32_{bf16,f16} for attention's scores, d = a b (first) and d += a b (next), with the register files named: a
+// wavefront alone on its SIMD has 256 registers that vector instructions can use and 256 more that only matrix instructions and
+// copies can, and the allocator, left to choose, puts the scores into the latter and copies every one of them back.  d is in
+// vector registers; b, which stays the same for a whole kernel, in accumulation registers.
+// The rules on the wait states around them are those of the comment at mfma_results_settle; NOPS: idle states in front, for an
+// operand that a vector instruction has just written (two are wanted).
+template <bool F16, bool NOPS = false> __device__ __forceinline__ void mfma16_first(const u32x4_t &a, const u32x4_t &b, f32x4_acc_t &d) {
+    if constexpr (F16 && NOPS) asm volatile("s_nop 1\n\tv_mfma_f32_16x16x32_f16 %0, %1, %2, 0" : "=&v"(d) : "v"(a), "a"(b));
+    else if constexpr (F16) asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, 0" : "=&v"(d) : "v"(a), "a"(b));
+    else if constexpr (NOPS) asm volatile("s_nop 1\n\tv_mfma_f32_16x16x32_bf16 %0, %1, %2, 0" : "=&v"(d) : "v"(a), "a"(b));
+    else asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, 0" : "=&v"(d) : "v"(a), "a"(b));
+}
+template <bool F16, bool NOPS = false> __device__ __forceinline__ void mfma16_next(const u32x4_t &a, const u32x4_t &b, f32x4_acc_t &d) {
+    if constexpr (F16 && NOPS) asm volatile("s_nop 1\n\tv_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+v"(d) : "v"(a), "a"(b));
+    else if constexpr (F16) asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+v"(d) : "v"(a), "a"(b));
+    else if constexpr (NOPS) asm volatile("s_nop 1\n\tv_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+v"(d) : "v"(a), "a"(b));
+    else asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+v"(d) : "v"(a), "a"(b));
+}
+// c *= s for an accumulator in accumulation registers, without moving it out of them for good (rarely executed; behind
+// mfma_results_settle, and with it between this and the next matrix instruction)
+__device__ __forceinline__ void scale4_acc(f32x4_acc_t &c, float s) {
+    float t;
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+        asm volatile("v_accvgpr_read_b32 %1, %0\n\ts_nop 1\n\tv_mul_f32 %1, %2, %1\n\ts_nop 1\n\tv_accvgpr_write_b32 %0, %1"
+                     : "+a"(c[e]), "=&v"(t) : "v"(s));
+}
+// an empty statement that takes and returns a value: it is there by then, and in this register file
+template <class T> __device__ __forceinline__ void pin_vector(T &v) { asm volatile("" : "+v"(v)); }
+template <class T> __device__ __forceinline__ void pin_accumulation(T &v) { asm volatile("" : "+a"(v)); }
+
 // v_mfma_scale_f32_16x16x128_f8f6f4 with unit scales (scale bytes 0x7F = 2^0), both operands of one 8-bit float format
 // (FMT 0 = e4m3, 1 = e5m2: the instruction's cbsz / blgp fields), the accumulator tied as above -- left to the register
 // allocator, kernels with this many small accumulators came out with copies inside the loop; an accumulator is next

@@ -109,8 +109,8 @@ extern "C" {
 int hodu_rocm_debug_force_tile(hodu_rocm_ctx *ctx, int tile) {
     if (!ctx) return fail(HODU_ROCM_INVALID_ARG, "context is null");
     const bool ok = tile == -1 || (tile >= 0 && tile <= 3) || (tile >= 10 && tile <= 16) || tile == 30 || tile == 31 ||
-                    (tile >= 32 && tile <= 34) || (tile >= 35 && tile <= 39) || (tile >= 40 && tile <= 43);
-    if (!ok) return fail(HODU_ROCM_INVALID_ARG, "tile %d not in -1..3, 10..16, 30..39, 40..43", tile);
+                    (tile >= 32 && tile <= 34) || (tile >= 35 && tile <= 39) || (tile >= 40 && tile <= 43) || (tile >= 50 && tile <= 52);
+    if (!ok) return fail(HODU_ROCM_INVALID_ARG, "tile %d not in -1..3, 10..16, 30..39, 40..43, 50..52", tile);
     std::lock_guard<std::recursive_mutex> hold(ctx->mu);
     ctx->force_tile = tile;
     return HODU_ROCM_OK;

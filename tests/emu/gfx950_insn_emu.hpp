@@ -326,6 +326,16 @@ inline void mfma16x16x32_bf16(const emu_u32x4 &a, const emu_u32x4 &b, f32x4_acc_
 inline void mfma16x16x32_f16(const emu_u32x4 &a, const emu_u32x4 &b, f32x4_acc_t &c) { emu::mfma_8k<16, emu::kMfmaF16>(a, b, c); }
 typedef int emu_i32x8 __attribute__((ext_vector_type(8)));
 template <int FMT> inline void mfma16x16x128_f8(const emu_i32x8 &a, const emu_i32x8 &b, f32x4_acc_t &c) { emu::mfma_f8<16, FMT>(a, b, c); }
+template <bool F16, bool NOPS = false> inline void mfma16_next(const emu_u32x4 &a, const emu_u32x4 &b, f32x4_acc_t &d) {
+    emu::mfma_8k<16, F16 ? emu::kMfmaF16 : emu::kMfmaBf16>(a, b, d);
+}
+template <bool F16, bool NOPS = false> inline void mfma16_first(const emu_u32x4 &a, const emu_u32x4 &b, f32x4_acc_t &d) {
+    for (int e = 0; e < 4; e++) d[e] = 0.f;
+    mfma16_next<F16>(a, b, d);
+}
+template <class T> inline void pin_vector(T &) {}
+template <class T> inline void pin_accumulation(T &) {}
+inline void scale4_acc(f32x4_acc_t &c, float s) { for (int e = 0; e < 4; e++) c[e] *= s; }
 inline void mfma_results_settle() {}
 
 inline void emu_set_m0(unsigned v) { EMU_M0 = v; EMU_M0_WRITTEN = true; }

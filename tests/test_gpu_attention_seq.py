@@ -11,6 +11,9 @@ pytestmark = pytest.mark.gpu
 HEADS = [(1, 1), (4, 2), (5, 1), (8, 1), (6, 6), (34, 2)]  # (query heads, key / value heads)
 
 
+TILES = [50, 51, 52]  # the kernels for tiles of 16, 128 and 192 or 256 rows
+
+
 @pytest.fixture(scope="module")
 def ctx():
     c = ffi.Context(0)
@@ -165,6 +168,32 @@ def test_refusals(ctx):
     ctx.attention_paged("bf16", q, kc, vc, out, off, table, lens, ffi.paged_attention_md(2, 8, 4, 2, 64, 0, 16, 4), bits)
     ctx.sync()
     assert not ctx.download(out, np.uint16)[:2 * 4 * 64].any()  # no page, no key: zeros
+
+
+@pytest.mark.parametrize("tile", TILES)
+@pytest.mark.parametrize("dt,cache_dt", [("bf16", "bf16"), ("f16", "f16"), ("bf16", "f8e4m3"), ("f16", "f8e4m3")])
+@pytest.mark.parametrize("d", [64, 128])
+def test_every_tile(ctx, tile, dt, cache_dt, d):
+    """each kernel on what the choice would not hand it: few rows, many short sequences, ragged ends of every stage"""
+    ctx.force_tile(tile)
+    try:
+        for n, (new, lens, hq, hk, page) in enumerate([([1, 1, 3], [1, 30, 70], 4, 2, 16), ([1, 9], [200, 129], 7, 1, 3), ([70, 2], [290, 64], 2, 2, 24),
+                                                       ([66], [391], 5, 1, 1), ([5, 0, 2], [3, 0, 257], 2, 1, 64)]):
+            S.run_paged(ctx, dt, new, lens, hq, hk, d, page, cache_dt, seed=200 + n)
+        S.run_paged(ctx, dt, [40, 3], [333, 95], 4, 2, d, 16, cache_dt, seed=210, garbage=0x7F if cache_dt == "f8e4m3" else 0x7F80)
+        if cache_dt == dt:
+            for causal in (True, False):
+                for n, (lens, hq, hk) in enumerate([([1, 2], 4, 2), ([65, 31, 100], 3, 1), ([0, 193, 1], 2, 2), ([330], 2, 1)]):
+                    S.run_varlen(ctx, dt, lens, lens, hq, hk, d, causal, seed=220 + n)
+                S.run_varlen(ctx, dt, [3, 40, 70], [260, 7, 65], 4, 2, d, causal, seed=230)
+
+            def ramp(q, k, v):
+                q[...] = np.abs(q)
+                k[...] = 0.3 * k + np.linspace(-3, 3, k.shape[0])[:, None, None]
+            S.run_varlen(ctx, dt, [420], [420], 2, 1, d, True, seed=231, edit=ramp)
+            S.run_varlen(ctx, dt, [3], [420], 2, 1, d, False, seed=232, edit=ramp)
+    finally:
+        ctx.force_tile(-1)
 
 
 def test_calls_in_a_row_give_the_same_bits(ctx):
