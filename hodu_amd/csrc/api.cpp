@@ -526,6 +526,7 @@ static int seq_attention_entry(const char *what, hodu_rocm_ctx *ctx, int dtype, 
     std::lock_guard<std::recursive_mutex> hold(ctx->mu);
     HODU_HIP(hipSetDevice(ctx->device));
     int rc = launch_seq_attention(ctx, dtype, cache_dtype, q, k, v, out, a);
+    if (rc == HODU_ROCM_HIP_ERROR || rc == HODU_ROCM_OOM) ctx->arrival_stale = true;
     if (rc == HODU_ROCM_UNSUPPORTED)
         return fail(HODU_ROCM_UNSUPPORTED, "%s: needs head dim 64 or 128, 16-byte aligned rows, heads and bases and a positive finite scale", what);
     return rc;

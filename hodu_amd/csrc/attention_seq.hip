@@ -13,6 +13,7 @@
 // and o / l at the end: one pass, scores never leave the chip.
 #include <type_traits>
 
+#include "agent_scope.hpp"
 #include "common.hpp"
 #include "device_types.hpp"
 #include "gemm_mfma_pipe.hpp"
@@ -45,18 +46,27 @@ __device__ __forceinline__ int quot(int n, const FixedDiv &f) { return (int)(((u
 __device__ __forceinline__ int from_lane(int v, int from) { return __builtin_amdgcn_ds_bpermute(from << 2, v); }
 
 // The sequence and first row of tile `tile` of `rows` rows (found by the whole wavefront, the same in all lanes); false
-// past the last tile.  n: the sequence's tokens, q0: its first one
-template <int ROWS> __device__ __forceinline__ bool find_tile(const DevSeq &a, int tile, int &b, int &row0, int &q0, int &n) {
+// past the last tile.  n: the sequence's tokens, q0: its first one; m: its keys and, packed, k0: where they begin
+struct SeqTile {
+    int b, row0, q0, n, k0, m;
+};
+template <int ROWS, bool PAGED> __device__ __forceinline__ bool find_tile(const DevSeq &a, int tile, SeqTile &f) {
     const int lane = threadIdx.x & 63;
     int before = 0;
     for (int base = 0; base < a.batch; base += 64) {
         const int s = base + lane;
-        int lo = 0, len = 0;
+        int lo = 0, len = 0, k0 = 0, m = 0;
         if (s < a.batch) {
-            lo = a.q_offsets[s];
-            const int hi = a.q_offsets[s + 1] < a.q_tokens ? a.q_offsets[s + 1] : a.q_tokens;
-            lo = lo > 0 ? lo : 0;
+            const int qa = a.q_offsets[s], qb = a.q_offsets[s + 1];
+            int ka = 0, kb;
+            if constexpr (PAGED) kb = a.lens[s];
+            else ka = a.k_offsets[s], kb = a.k_offsets[s + 1];
+            const int hi = qb < a.q_tokens ? qb : a.q_tokens;
+            lo = qa > 0 ? qa : 0;
             len = hi > lo ? hi - lo : 0;
+            const int k_most = PAGED ? a.width * a.page.d : a.k_tokens, k_hi = kb < k_most ? kb : k_most;
+            k0 = ka > 0 ? ka : 0;
+            m = k_hi > k0 ? k_hi - k0 : 0;
         }
         const int tiles = (int)(((long)len * a.group + ROWS - 1) / ROWS);
         int sum = tiles;  // inclusive over the lanes
@@ -69,37 +79,19 @@ template <int ROWS> __device__ __forceinline__ bool find_tile(const DevSeq &a, i
         if (tile < before + all) {
             const unsigned long long past = __builtin_amdgcn_ballot_w64(before + sum > tile);
             const int at = __builtin_ctzll(past);
-            b = base + at;
             const int first = before + from_lane(sum, at) - from_lane(tiles, at);
-            q0 = from_lane(lo, at);
-            n = from_lane(len, at);
-            row0 = (tile - first) * ROWS;
-            b = __builtin_amdgcn_readfirstlane(b);
-            q0 = __builtin_amdgcn_readfirstlane(q0);
-            n = __builtin_amdgcn_readfirstlane(n);
-            row0 = __builtin_amdgcn_readfirstlane(row0);
+            f.b = __builtin_amdgcn_readfirstlane(base + at);
+            f.q0 = __builtin_amdgcn_readfirstlane(from_lane(lo, at));
+            f.n = __builtin_amdgcn_readfirstlane(from_lane(len, at));
+            f.k0 = __builtin_amdgcn_readfirstlane(from_lane(k0, at));
+            f.m = __builtin_amdgcn_readfirstlane(from_lane(m, at));
+            f.row0 = __builtin_amdgcn_readfirstlane((tile - first) * ROWS);
             // (offsets that do not ascend can make the count above wrap; a tile outside its sequence is no tile)
-            return row0 >= 0 && row0 < (long)n * a.group;
+            return f.row0 >= 0 && f.row0 < (long)f.n * a.group;
         }
         before += all;
     }
     return false;
-}
-
-// keys of sequence b and, packed, where they begin
-template <bool PAGED> __device__ __forceinline__ void find_keys(const DevSeq &a, int b, int &k0, int &m) {
-    if constexpr (PAGED) {
-        k0 = 0;
-        const int most = a.width * a.page.d, len = a.lens[b];
-        m = len < 0 ? 0 : len < most ? len : most;
-    } else {
-        k0 = a.k_offsets[b];
-        const int hi = a.k_offsets[b + 1] < a.k_tokens ? a.k_offsets[b + 1] : a.k_tokens;
-        k0 = k0 > 0 ? k0 : 0;
-        m = hi > k0 ? hi - k0 : 0;
-    }
-    k0 = __builtin_amdgcn_readfirstlane(k0);
-    m = __builtin_amdgcn_readfirstlane(m);
 }
 
 template <int CK> __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
@@ -125,14 +117,22 @@ template <int CK> __device__ __forceinline__ u32x4_t widen8(const u32x2_t &v) {
     }
 }
 
-// ---- tiles of 16 rows, one wavefront at a time over a range of the keys -------------------------------------------------
-// A workgroup is four wavefronts with the same 16 rows and a quarter of the keys each, 32 keys at a step; they meet once, at the end, in
-// LDS.  S^T = K Q^T and O^T += V^T P^T on 16 x 16 x 32: a lane then owns one row throughout (column lane % 16).  The rows
+// ---- tiles of 16 rows: single tokens and short chunks ---------------------------------------------------------------------
+// Bound by the cache's bytes, or, where there are few of them, by latency.  A workgroup is four wavefronts with the same 16
+// rows; the keys of a tile are cut into ranges of 32-key blocks, one per wavefront of each of the tile's workgroups, so that a single long
+// sequence still reaches every compute unit.  A wavefront has an LDS ring of its own (32 KB: the next block or blocks are in flight while it computes,
+// 64 KB and more per compute unit), meets nobody until its range is done, and there is no barrier in the loop.
+//
+// S^T = K Q^T and O^T += V^T P^T on 16 x 16 x 32: a lane then owns one row throughout (column lane % 16).  The rows
 // of the first product's left operand are keys in the order 8 (r / 4) + 4 t + r % 4 for tile t of two, so that a lane's
 // eight scores are those of 8 consecutive keys -- which is the operand layout of P in the second product, and the order
 // in which the LDS transpose reads deliver V's keys.  K and V blocks go from memory into LDS without registers in between,
 // rows back to back, 16-byte chunks XOR-swizzled on the source side so that the rows of one read fall into different banks.
-constexpr int R16 = 16, R16_NT = 256, R16_BK = 32;
+//
+// A tile's workgroups meet through the workspace (agent_scope.hpp): each leaves its rows' (reference, sum, O), the last one
+// to arrive adds them in range order, so the result does not depend on who was last.
+constexpr int R16 = 16, R16_NT = 256, R16_BK = 32, R16_WINDOW = 256;
+constexpr int R16_MIN_BLOCKS = 4;  // blocks of a workgroup below which keys are not cut further: one per wavefront
 template <int D, bool F8> struct R16Geom {
     static_assert(D == 64 || D == 128, "head dim");
     static constexpr int ES = F8 ? 1 : 2, ROW = D * ES, CPR = ROW / 16, BLOCK = R16_BK * ROW, DMAS = BLOCK / 1024, KPI = 64 / CPR;
@@ -149,26 +149,30 @@ template <int D, bool F8> struct R16Geom {
         const int bits = (key & 3) | ((key >> 1) & 4);
         return (ROW == 256 ? bits : bits >> 1) << 1;
     }
-    static constexpr int WAVE = 2 * BLOCK;                   // a wavefront's K and V block
-    static constexpr int MERGE = 4 * R16 * (D + 4) * 4;      // (m, l, O) of four wavefronts
-    static constexpr int LDS = 4 * WAVE > MERGE ? 4 * WAVE : MERGE;
+    static constexpr int RING = BLOCK == 8192 ? 2 : 4;       // blocks of K and of V in a wavefront's ring
+    static constexpr int WAVE = RING * 2 * BLOCK;
+    static constexpr int LINE = D + 4;                       // floats of a row's (reference, sum, -, -, O)
+    static constexpr int MERGE = 4 * R16 * LINE * 4;
+    static constexpr int WINDOW_AT = 4 * WAVE > MERGE ? 4 * WAVE : MERGE;
+    static constexpr int LDS = WINDOW_AT + 4 * R16_WINDOW * 4 + 16;
 };
 
 template <int CK, int D, bool PAGED, bool F8>
 __global__ __launch_bounds__(R16_NT) void seq_attention_r16_kernel(const uint16_t *__restrict__ Q, const char *__restrict__ K,
-                                                                   const char *__restrict__ V, uint16_t *__restrict__ O, DevSeq a) {
+                                                                   const char *__restrict__ V, uint16_t *__restrict__ O, DevSeq a,
+                                                                   float *ws, unsigned ws_bytes, int *arrival) {
     typedef R16Geom<D, F8> G;
     typedef Compute<CK> Cmp;
     typedef typename Cmp::acc_t acc_t;
+    constexpr bool F16 = CK == mfma::CK_F16;
     HODU_DYNAMIC_LDS(smem);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 15, g = lane >> 4;
     const int kvh = blockIdx.x % a.kv_heads;
-    int b, row0, q0, n, k0, m;
-    if (!find_tile<R16>(a, blockIdx.x / a.kv_heads, b, row0, q0, n)) return;
-    find_keys<PAGED>(a, b, k0, m);
+    SeqTile f;
+    if (!find_tile<R16, PAGED>(a, blockIdx.x / a.kv_heads, f)) return;
+    const int row0 = f.row0, q0 = f.q0, n = f.n, m = f.m, rows = n * a.group;
 
     // the lane's row; rows past the sequence's last repeat it and are not stored
-    const int rows = n * a.group;
     const int rr = row0 + r < rows ? row0 + r : rows - 1;
     const int tok = quot(rr, a.by_group), head = kvh * a.group + rr - tok * a.group;
     const int open = a.causal ? tok + m - n + 1 : m;  // keys the row attends, <= 0: none
@@ -176,29 +180,41 @@ __global__ __launch_bounds__(R16_NT) void seq_attention_r16_kernel(const uint16_
     const int keys = a.causal ? last_tok + m - n + 1 : m;          // keys the tile needs
     const int all_open = a.causal ? first_tok + m - n + 1 : m;     // keys below this are open to every row
     const int blocks = keys > 0 ? (keys + R16_BK - 1) / R16_BK : 0;
-    const int blk0 = (int)((long)blocks * wave / 4), blk1 = (int)((long)blocks * (wave + 1) / 4);
+    // the tile's workgroups: as many as the launch has for it and the keys are worth
+    const int worth = (blocks + R16_MIN_BLOCKS - 1) / R16_MIN_BLOCKS;
+    const int splits = worth < 1 ? 1 : worth < (int)gridDim.y ? worth : (int)gridDim.y;
+    const int split = blockIdx.y;
+    if (split >= splits) return;
+    const int blk0 = (int)((long)blocks * (split * 4 + wave) / (splits * 4)), blk1 = (int)((long)blocks * (split * 4 + wave + 1) / (splits * 4));
 
     u32x4_t qf[G::KS];
 #pragma unroll
     for (int ks = 0; ks < G::KS; ks++)
         qf[ks] = *reinterpret_cast<const u32x4_t *>(Q + (q0 + tok) * a.q_token + head * a.q_head + 32 * ks + 8 * g);
     const float c = a.scale_log2e * (F8 ? a.k_scale[kvh] : 1.f);
+    const float v_scale = F8 ? a.v_scale[kvh] : 1.f;
 
-    char *kl = smem + wave * G::WAVE, *vl = kl + G::BLOCK;
-    const unsigned kl0 = (unsigned)(uintptr_t)kl, vl0 = (unsigned)(uintptr_t)vl;
+    char *ring = smem + wave * G::WAVE;
+    const unsigned ring0 = (unsigned)(uintptr_t)ring;
     const char *kbase = K + kvh * a.kc.head, *vbase = V + kvh * a.vc.head;
-    int k_frag[2];
-#pragma unroll
-    for (int t = 0; t < 2; t++) k_frag[t] = 8 * (r >> 2) + 4 * t + (r & 3);
-    acc_t o[G::DT];
-#pragma unroll
-    for (int j = 0; j < G::DT; j++) o[j] = acc_t{0.f, 0.f, 0.f, 0.f};
-    float m_run = -INFINITY, l_run = 0.f;
-
-    for (int blk = blk0; blk < blk1; blk++) {
-        // the last block's reads have been answered before this one's loads are issued
-        __builtin_amdgcn_s_waitcnt(mfma::waitcnt_vm_lgkm0(63));
+    int *window = reinterpret_cast<int *>(smem + G::WINDOW_AT) + wave * R16_WINDOW;  // the wavefront's next table entries
+    int window0 = 0;
+    [[maybe_unused]] auto fill_window = [&](int from) __attribute__((always_inline)) {
+        const int cols = quot(keys - 1, a.page) + 1;
         mfma::wave_lds_fence();
+#pragma unroll
+        for (int i = 0; i < R16_WINDOW / 64; i++) {
+            const int col = from + i * 64 + lane, pg = a.table[(long)f.b * a.width + (col < cols ? col : cols - 1)];
+            window[i * 64 + lane] = pg < 0 ? 0 : pg < a.n_pages ? pg : a.n_pages - 1;
+        }
+        window0 = from;
+        mfma::wave_lds_fence();
+    };
+    auto issue = [&](int blk, int slot) __attribute__((always_inline)) {
+        if constexpr (PAGED) {
+            const int last = (blk + 1) * R16_BK < keys ? (blk + 1) * R16_BK - 1 : keys - 1;
+            if (quot(last, a.page) - window0 >= R16_WINDOW) fill_window(quot(blk * R16_BK, a.page));
+        }
 #pragma unroll
         for (int i = 0; i < G::DMAS; i++) {
             const int kk = i * G::KPI + lane / G::CPR;  // the lane's key of this instruction
@@ -206,27 +222,51 @@ __global__ __launch_bounds__(R16_NT) void seq_attention_r16_kernel(const uint16_
             key = key < keys ? key : keys - 1;  // behind the last key: that one again, masked below
             long ko, vo;
             if constexpr (PAGED) {
-                const int col = quot(key, a.page), in = key - col * a.page.d;
-                int pg = a.table[(long)b * a.width + col];
-                pg = pg < 0 ? 0 : pg < a.n_pages ? pg : a.n_pages - 1;
+                const int col = quot(key, a.page), in = key - col * a.page.d, pg = window[col - window0];
                 ko = pg * a.kc.page + in * a.kc.token;
                 vo = pg * a.vc.page + in * a.vc.token;
             } else {
-                ko = (k0 + key) * a.kc.token;
-                vo = (k0 + key) * a.vc.token;
+                ko = (f.k0 + key) * a.kc.token;
+                vo = (f.k0 + key) * a.vc.token;
             }
-            const int slot = lane % G::CPR;
-            mfma::dma16_raw(kbase + ko + ((slot ^ G::kswz(kk)) << 4), __builtin_amdgcn_readfirstlane(kl0 + i * 1024));
-            mfma::dma16_raw(vbase + vo + ((slot ^ G::vswz(kk)) << 4), __builtin_amdgcn_readfirstlane(vl0 + i * 1024));
+            const int at = lane % G::CPR;
+            const unsigned to = ring0 + slot * 2 * G::BLOCK + i * 1024;
+            mfma::dma16_raw(kbase + ko + ((at ^ G::kswz(kk)) << 4), __builtin_amdgcn_readfirstlane(to));
+            mfma::dma16_raw(vbase + vo + ((at ^ G::vswz(kk)) << 4), __builtin_amdgcn_readfirstlane(to + G::BLOCK));
         }
-        __builtin_amdgcn_s_waitcnt(mfma::waitcnt_vm_lgkm0(0));
+    };
+
+    acc_t o[G::DT];
+#pragma unroll
+    for (int j = 0; j < G::DT; j++) o[j] = acc_t{0.f, 0.f, 0.f, 0.f};
+    // the exponent reference, an integer that moves only when a score exceeds it by 2^SLACK: see the wide kernel below
+    constexpr float SLACK = F16 ? 12.f : 64.f;
+    float e_ref = -1e30f, l_run = 0.f;
+    if (blk0 < blk1) {
+        if constexpr (PAGED) fill_window(quot(blk0 * R16_BK, a.page));
+        // (pinned: these loads have returned before the ones are issued that the compiler does not know of)
+#pragma unroll
+        for (int ks = 0; ks < G::KS; ks++) mfma::pin_vector(qf[ks]);
+#pragma unroll
+        for (int s = 0; s < G::RING; s++)
+            if (blk0 + s < blk1) issue(blk0 + s, s);
+    }
+    int slot = 0;
+    for (int blk = blk0; blk < blk1; blk++) {
+        // this block has landed, up to RING - 1 later ones may be in flight
+        const int later = blk1 - 1 - blk;
+        if (later >= G::RING - 1) __builtin_amdgcn_s_waitcnt(mfma::waitcnt_vm_lgkm0((G::RING - 1) * 2 * G::DMAS));
+        else if (G::RING > 2 && later == 2) __builtin_amdgcn_s_waitcnt(mfma::waitcnt_vm_lgkm0(2 * 2 * G::DMAS));
+        else if (G::RING > 2 && later == 1) __builtin_amdgcn_s_waitcnt(mfma::waitcnt_vm_lgkm0(2 * G::DMAS));
+        else __builtin_amdgcn_s_waitcnt(mfma::waitcnt_vm_lgkm0(0));
         mfma::wave_lds_fence();
+        const char *kl = ring + slot * 2 * G::BLOCK, *vl = kl + G::BLOCK;
 
         acc_t s[2];
 #pragma unroll
         for (int t = 0; t < 2; t++) {
             s[t] = acc_t{0.f, 0.f, 0.f, 0.f};
-            const int key = k_frag[t];
+            const int key = 8 * (r >> 2) + 4 * t + (r & 3);
 #pragma unroll
             for (int ks = 0; ks < G::KS; ks++) {
                 u32x4_t kf;
@@ -245,22 +285,27 @@ __global__ __launch_bounds__(R16_NT) void seq_attention_r16_kernel(const uint16_
 #pragma unroll
             for (int e = 0; e < 8; e++) sv[e] = blk * R16_BK + 8 * g + e < open ? sv[e] : -INFINITY;
         }
-        float mx = sv[0];
+        float top = sv[0];
 #pragma unroll
-        for (int e = 1; e < 8; e++) mx = __builtin_fmaxf(mx, sv[e]);
-        mx = __builtin_fmaxf(mx, __shfl_xor(mx, 16));
-        mx = __builtin_fmaxf(mx, __shfl_xor(mx, 32));
-        const float m_new = __builtin_fmaxf(m_run, mx);
-        const float m_use = m_new == -INFINITY ? 0.f : m_new;  // no key yet: 2^(-inf) = 0 keeps the sums at zero
-        const float keep = __builtin_amdgcn_exp2f((m_run - m_use) * c);
-        m_run = m_new;
-        float p[8], sum = 0.f;
+        for (int e = 1; e < 8; e++) top = __builtin_fmaxf(top, sv[e]);
+        if (__builtin_amdgcn_ballot_w64(c * top > e_ref + SLACK) != 0) {
+            top = __builtin_fmaxf(top, __shfl_xor(top, 16));
+            top = c * __builtin_fmaxf(top, __shfl_xor(top, 32));
+            const float e_new = top > e_ref + SLACK ? ceilf(top) : e_ref;
+            const float keep = __builtin_amdgcn_exp2f(e_ref - e_new);
+            e_ref = e_new;
+            l_run *= keep;
+#pragma unroll
+            for (int j = 0; j < G::DT; j++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) o[j][e] *= keep;
+        }
+        float p[8];
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-            p[e] = __builtin_amdgcn_exp2f((sv[e] - m_use) * c);
-            sum += p[e];
+            p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[e], c, -e_ref));
+            l_run += p[e];  // the lane's share; the row's four lanes add up at the end
         }
-        l_run = l_run * keep + sum;  // the lane's share; the row's four lanes add up at the end
         const u32x4_t pf = {pack2<CK>(p[0], p[1]), pack2<CK>(p[2], p[3]), pack2<CK>(p[4], p[5]), pack2<CK>(p[6], p[7])};
 #pragma unroll
         for (int j = 0; j < G::DT; j++) {
@@ -274,22 +319,26 @@ __global__ __launch_bounds__(R16_NT) void seq_attention_r16_kernel(const uint16_
                 const u32x2_t hi = lds_get_tr<2>(vl, (key + 4) * G::ROW + ((ch ^ G::vswz(key + 4)) << 4) + (r & 1) * 8);
                 vf = u32x4_t{lo.x, lo.y, hi.x, hi.y};
             }
-#pragma unroll
-            for (int e = 0; e < 4; e++) o[j][e] *= keep;
             Cmp::mma(vf, pf, o[j]);
         }
+        if (blk + G::RING < blk1) {
+            // the block's reads have been answered before its slot's next loads are issued
+            __builtin_amdgcn_s_waitcnt(mfma::waitcnt_vm_lgkm0(63));
+            mfma::wave_lds_fence();
+            issue(blk + G::RING, slot);
+        }
+        slot = slot + 1 < G::RING ? slot + 1 : 0;
     }
 
-    // ---- the four wavefronts meet: per wavefront and row (m, l, -, -, O) ----
+    // ---- the four wavefronts meet: per wavefront and row (reference, sum, -, -, O) ----
     l_run += __shfl_xor(l_run, 16);
     l_run += __shfl_xor(l_run, 32);
     __syncthreads();
-    constexpr int LINE = D + 4;
     float *mg = reinterpret_cast<float *>(smem);
     {
-        float *mine = mg + (wave * R16 + r) * LINE;
+        float *mine = mg + (wave * R16 + r) * G::LINE;
         if (g == 0) {
-            mine[0] = m_run;
+            mine[0] = e_ref;
             mine[1] = l_run;
         }
 #pragma unroll
@@ -297,33 +346,53 @@ __global__ __launch_bounds__(R16_NT) void seq_attention_r16_kernel(const uint16_
     }
     __syncthreads();
     const int row = tid >> 4, part = tid & 15;  // 16 threads a row, D / 16 elements each
-    if (row0 + row >= rows) return;
-    float mx = -INFINITY, l = 0.f, w[4];
+    constexpr int PER = D / 16;
+    float e_all = -1e30f, l = 0.f, x[PER];
 #pragma unroll
-    for (int i = 0; i < 4; i++) mx = __builtin_fmaxf(mx, mg[(i * R16 + row) * LINE]);
-    const float c2 = c;
+    for (int i = 0; i < 4; i++) e_all = __builtin_fmaxf(e_all, mg[(i * R16 + row) * G::LINE]);
+#pragma unroll
+    for (int e = 0; e < PER; e++) x[e] = 0.f;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        const float *line = mg + (i * R16 + row) * LINE;
-        w[i] = line[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((line[0] - mx) * c2);
-        l += line[1] * w[i];
+        const float *line = mg + (i * R16 + row) * G::LINE;
+        const float w = __builtin_amdgcn_exp2f(line[0] - e_all);
+        l += line[1] * w;
+#pragma unroll
+        for (int e = 0; e < PER; e++) x[e] += line[4 + part * PER + e] * w;
     }
-    // a row without keys: l = 0, and zero is what it gives
-    const float inv = l == 0.f ? 0.f : (F8 ? a.v_scale[kvh] : 1.f) / l;
+    if (splits > 1) {
+        const __amdgpu_buffer_rsrc_t buf = agent_buffer(ws, ws_bytes);
+        const unsigned tile_at = blockIdx.x * gridDim.y * R16 * G::LINE * 4, mine = tile_at + (split * R16 + row) * G::LINE * 4;
+        if (part == 0) store16_agent(buf, mine, f32x4_t{e_all, l, 0.f, 0.f});
+#pragma unroll
+        for (int e = 0; e < PER; e += 4) store16_agent(buf, mine + (4 + part * PER + e) * 4, f32x4_t{x[e], x[e + 1], x[e + 2], x[e + 3]});
+        int *flag = reinterpret_cast<int *>(smem + G::WINDOW_AT + 4 * R16_WINDOW * 4);
+        if (!arrive_and_check_last(arrival + blockIdx.x, splits, flag, tid)) return;
+        e_all = -1e30f;
+        for (int i = 0; i < splits; i++) e_all = __builtin_fmaxf(e_all, load16_agent<f32x4_t>(buf, tile_at + (i * R16 + row) * G::LINE * 4).x);
+        l = 0.f;
+#pragma unroll
+        for (int e = 0; e < PER; e++) x[e] = 0.f;
+        for (int i = 0; i < splits; i++) {
+            const unsigned at = tile_at + (i * R16 + row) * G::LINE * 4;
+            const f32x4_t h = load16_agent<f32x4_t>(buf, at);
+            const float w = __builtin_amdgcn_exp2f(h.x - e_all);
+            l += h.y * w;
+#pragma unroll
+            for (int e = 0; e < PER; e += 4) {
+                const f32x4_t y = load16_agent<f32x4_t>(buf, at + (4 + part * PER + e) * 4);
+#pragma unroll
+                for (int q = 0; q < 4; q++) x[e + q] += y[q] * w;
+            }
+        }
+        arrival_reset(arrival + blockIdx.x, tid);
+    }
+    if (row0 + row >= rows) return;
+    const float inv = l == 0.f ? 0.f : v_scale / l;  // a row without keys: l = 0, and zero is what it gives
     const int wtok = quot(row0 + row, a.by_group), whead = kvh * a.group + row0 + row - wtok * a.group;
-    constexpr int PER = D / 16;
     uint32_t out[PER / 2];
 #pragma unroll
-    for (int e = 0; e < PER; e += 2) {
-        float x = 0.f, y = 0.f;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const float *line = mg + (i * R16 + row) * LINE + 4 + part * PER + e;
-            x += line[0] * w[i];
-            y += line[1] * w[i];
-        }
-        out[e / 2] = pack2<CK>(x * inv, y * inv);
-    }
+    for (int e = 0; e < PER; e += 2) out[e / 2] = pack2<CK>(x[e] * inv, x[e + 1] * inv);
     uint16_t *dst = O + ((long)(q0 + wtok) * a.heads + whead) * D + part * PER;
     if constexpr (PER == 8) *reinterpret_cast<u32x4_t *>(dst) = u32x4_t{out[0], out[1], out[2], out[3]};
     else *reinterpret_cast<u32x2_t *>(dst) = u32x2_t{out[0], out[1]};
@@ -370,11 +439,9 @@ __global__ __launch_bounds__(W_NT, 1) void seq_attention_wide_kernel(const uint1
     const unsigned lds0 = (unsigned)(uintptr_t)smem;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 15, g = lane >> 4;
     const int kvh = blockIdx.x % a.kv_heads;
-    int b, row0, q0, n, k0, m;
-    if (!find_tile<BM>(a, blockIdx.x / a.kv_heads, b, row0, q0, n)) return;
-    find_keys<PAGED>(a, b, k0, m);
-
-    const int rows = n * a.group;
+    SeqTile f;
+    if (!find_tile<BM, PAGED>(a, blockIdx.x / a.kv_heads, f)) return;
+    const int b = f.b, row0 = f.row0, q0 = f.q0, n = f.n, k0 = f.k0, m = f.m, rows = n * a.group;
     // the lane's rows, one per tile; rows past the sequence's last repeat it and are not stored
     int open[RT];
     u32x4_t qf[RT][KS];
@@ -782,8 +849,28 @@ int launch_seq_attention(hodu_rocm_ctx *ctx, int dtype, int cache_dtype, const v
         if (pin == 51 || (pin < 50 && avg_rows >= 48))
             return launch(seq_attention_wide_kernel<CK, D, PAGED, F8, 2>, 128, W_NT, WGeom<D, F8, PAGED>::LDS,
                           !PAGED ? "attention_varlen_wide128" : F8 ? "attention_paged_wide128_f8" : "attention_paged_wide128");
-        return launch(seq_attention_r16_kernel<CK, D, PAGED, F8>, R16, R16_NT, R16Geom<D, F8>::LDS,
-                      !PAGED ? "attention_varlen_r16" : F8 ? "attention_paged_r16_f8" : "attention_paged_r16");
+        // Few tiles over long contexts: the keys are cut across workgroups, to about eight per compute unit (they differ in
+        // length, and the last ones of a launch should be short).  How many of them a tile uses goes by its keys, on the device.
+        typedef R16Geom<D, F8> G;
+        const long tiles = (sequences + g.q_tokens * a.group / R16) * g.kv_heads;
+        const long most_keys = PAGED ? (long)a.width * a.page.d : g.k_tokens;
+        long splits = 8L * ctx->props.multiProcessorCount / tiles;
+        const long worth = (most_keys / R16_BK + R16_MIN_BLOCKS) / R16_MIN_BLOCKS;
+        splits = splits > worth ? worth : splits;
+        splits = splits > 64 ? 64 : splits;
+        if (splits < 1 || tiles > kArrivalSlots) splits = 1;
+        const size_t ws_bytes = splits > 1 ? (size_t)tiles * splits * R16 * G::LINE * 4 : 0;
+        if (splits > 1) {
+            if (int rc = ensure_workspace(ctx, ws_bytes)) return rc;
+            if (int rc = ensure_arrival(ctx)) return rc;
+        }
+        const auto kernel = seq_attention_r16_kernel<CK, D, PAGED, F8>;
+        if (tiles > 0x7FFFFFFFL) return HODU_ROCM_UNSUPPORTED;
+        if (int rc = ensure_dynamic_lds(ctx, reinterpret_cast<const void *>(kernel), G::LDS)) return rc;
+        ctx->last_kernel = !PAGED ? "attention_varlen_r16" : F8 ? "attention_paged_r16_f8" : "attention_paged_r16";
+        hipLaunchKernelGGL(kernel, dim3((unsigned)tiles, (unsigned)splits), dim3(R16_NT), G::LDS, ctx->stream, qp, kp, vp, (uint16_t *)out, a,
+                           (float *)ctx->workspace.ptr, (unsigned)ws_bytes, ctx->arrival);
+        return HODU_ROCM_OK;
     };
     auto by_type = [&](auto ck, auto d) -> int {
         if (!g.paged) return by_form(ck, d, std::false_type(), std::false_type());
