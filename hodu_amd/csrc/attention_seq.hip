@@ -126,36 +126,56 @@ template <int CK> __device__ __forceinline__ u32x4_t widen8(const u32x2_t &v) {
 // S^T = K Q^T and O^T += V^T P^T on 16 x 16 x 32: a lane then owns one row throughout (column lane % 16).  The rows
 // of the first product's left operand are keys in the order 8 (r / 4) + 4 t + r % 4 for tile t of two, so that a lane's
 // eight scores are those of 8 consecutive keys -- which is the operand layout of P in the second product, and the order
-// in which the LDS transpose reads deliver V's keys.  K and V blocks go from memory into LDS without registers in between,
-// rows back to back, 16-byte chunks XOR-swizzled on the source side so that the rows of one read fall into different banks.
+// in which the LDS transpose reads deliver V's keys.  K and V blocks go from memory into LDS without registers in between.
 //
 // A tile's workgroups meet through the workspace (agent_scope.hpp): each leaves its rows' (reference, sum, O), the last one
 // to arrive adds them in range order, so the result does not depend on who was last.
 constexpr int R16 = 16, R16_NT = 256, R16_BK = 32, R16_WINDOW = 256;
 constexpr int R16_MIN_BLOCKS = 4;  // blocks of a workgroup below which keys are not cut further: one per wavefront
-template <int D, bool F8> struct R16Geom {
+template <int D, bool F8> struct SeqGeom {
     static_assert(D == 64 || D == 128, "head dim");
-    static constexpr int ES = F8 ? 1 : 2, ROW = D * ES, CPR = ROW / 16, BLOCK = R16_BK * ROW, DMAS = BLOCK / 1024, KPI = 64 / CPR;
+    static constexpr int ES = F8 ? 1 : 2, ROW = D * ES, CPR = ROW / 16, KPI = 64 / CPR;  // bytes and 16-byte chunks of a row, keys of an LDS-DMA instruction
+    static constexpr int DMAS = 32 / KPI;           // instructions of a block of 32 keys, 1 KB each
     static constexpr int KS = D / 32, DT = D / 16;  // 32-wide slices of the head dim, 16-wide tiles of the output
-    // A read's lanes go through keys that differ in bits {0, 1, 3, 4} (K: 16 keys of a tile, one chunk each), {0, 1, 3} (V, 16-bit:
-    // 8 keys, two chunks each), {0, 1, 2, 3} (V, 8-bit: 16 keys, a chunk each); the lowest bits choose the row's part of the
-    // 64 banks already (256 / ROW rows lie side by side), the others go into the chunk index
-    static __device__ __forceinline__ int kswz(int key) {
-        const int bits = (key & 3) | ((key >> 1) & 12);
-        return ROW == 256 ? bits : ROW == 128 ? bits >> 1 : bits >> 2;
-    }
+    // Bank conflicts.  A K read's 16 lanes go through keys that differ in bits {0, 1, 3, 4}, one chunk each; a V read's 32 lanes through keys
+    // that differ in bits {0, 1, 3}, two chunks each (16-bit), or {0, 1, 2, 3}, a chunk each (8-bit).  Keys of one instruction are told
+    // apart by an XOR on the chunk index (on the source side), instructions by padding between them; the XOR stays below the bits that
+    // step along the head dim in K, so one address per lane serves all of K's fragments, and VB of them V's.
+    static constexpr int PADDED_K = 1024 + 32, PADDED_V = 1024 + 64;
+    static constexpr int BLOCK_K = DMAS * PADDED_K, BLOCK_V = DMAS * PADDED_V;  // 32 keys
+    static __device__ __forceinline__ int kswz(int key) { return ROW == 256 ? key & 3 : ROW == 128 ? (key >> 1) & 1 : (key >> 3) & 1; }
     static __device__ __forceinline__ int vswz(int key) {
-        if (F8) return ROW == 128 ? (key >> 1) & 7 : (key >> 2) & 3;
-        const int bits = (key & 3) | ((key >> 1) & 4);
-        return (ROW == 256 ? bits : bits >> 1) << 1;
+        if (F8) return ROW == 128 ? (key >> 1) & 3 : (key >> 2) & 3;
+        return (ROW == 256 ? key & 3 : (key >> 1) & 1) << 1;
     }
-    static constexpr int RING = BLOCK == 8192 ? 2 : 4;       // blocks of K and of V in a wavefront's ring
-    static constexpr int WAVE = RING * 2 * BLOCK;
+    // K fragment q = 2 ks + t: 16 keys of tile t, 32 of the head dim
+    static constexpr int KF = 2 * KS, K_STEP = 32 * ES, K_TILE = KPI == 4 ? PADDED_K : 4 * ROW;
+    static __device__ __forceinline__ int k_lane(int r, int g) {
+        const int key = 8 * (r >> 2) + (r & 3);
+        return key / KPI * PADDED_K + key % KPI * ROW + (((F8 ? g >> 1 : g) ^ kswz(key)) << 4) + (F8 ? (g & 1) * 8 : 0);
+    }
+    // V fragment j: 32 keys, 16 of the head dim, in VR transpose reads
+    static constexpr int VR = F8 ? 1 : 2, VB = F8 || D == 128 ? 4 : 2, V_STEP = VB * (F8 ? 16 : 32), V_HALF = KPI == 4 ? PADDED_V : 4 * ROW;
+    static __device__ __forceinline__ int v_lane(int r, int g, int b) {
+        const int key = 8 * g + (F8 ? r >> 1 : r >> 2);
+        return key / KPI * PADDED_V + key % KPI * ROW + (((F8 ? b : 2 * b + ((r >> 1) & 1)) ^ vswz(key)) << 4) + (r & 1) * 8;
+    }
+};
+template <int D, bool F8> struct R16Geom : SeqGeom<D, F8> {
+    typedef SeqGeom<D, F8> S;
+    static constexpr int RING = S::DMAS == 8 ? 2 : 4;        // blocks of K and of V in a wavefront's ring
+    static constexpr int BLOCK = S::BLOCK_K + S::BLOCK_V, WAVE = RING * BLOCK;
     static constexpr int LINE = D + 4;                       // floats of a row's (reference, sum, -, -, O)
     static constexpr int MERGE = 4 * R16 * LINE * 4;
     static constexpr int WINDOW_AT = 4 * WAVE > MERGE ? 4 * WAVE : MERGE;
     static constexpr int LDS = WINDOW_AT + 4 * R16_WINDOW * 4 + 16;
 };
+// 1.0 in every element: the row sums are one more tile of the second product, over the P that it multiplies (which is rounded,
+// so that the weights sum to one), and cost no vector instruction and no exchange between a row's lanes
+template <int CK> __device__ __forceinline__ u32x4_t ones() {
+    const uint32_t w = CK == mfma::CK_BF16 ? 0x3F803F80u : 0x3C003C00u;
+    return u32x4_t{w, w, w, w};
+}
 
 template <int CK, int D, bool PAGED, bool F8>
 __global__ __launch_bounds__(R16_NT) void seq_attention_r16_kernel(const uint16_t *__restrict__ Q, const char *__restrict__ K,
@@ -230,18 +250,23 @@ __global__ __launch_bounds__(R16_NT) void seq_attention_r16_kernel(const uint16_
                 vo = (f.k0 + key) * a.vc.token;
             }
             const int at = lane % G::CPR;
-            const unsigned to = ring0 + slot * 2 * G::BLOCK + i * 1024;
-            mfma::dma16_raw(kbase + ko + ((at ^ G::kswz(kk)) << 4), __builtin_amdgcn_readfirstlane(to));
-            mfma::dma16_raw(vbase + vo + ((at ^ G::vswz(kk)) << 4), __builtin_amdgcn_readfirstlane(to + G::BLOCK));
+            const unsigned to = ring0 + slot * G::BLOCK;
+            mfma::dma16_raw(kbase + ko + ((at ^ G::kswz(kk)) << 4), __builtin_amdgcn_readfirstlane(to + i * G::PADDED_K));
+            mfma::dma16_raw(vbase + vo + ((at ^ G::vswz(kk)) << 4), __builtin_amdgcn_readfirstlane(to + G::BLOCK_K + i * G::PADDED_V));
         }
     };
 
-    acc_t o[G::DT];
+    acc_t o[G::DT + 1];  // the last tile: the row sums
 #pragma unroll
-    for (int j = 0; j < G::DT; j++) o[j] = acc_t{0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j <= G::DT; j++) o[j] = acc_t{0.f, 0.f, 0.f, 0.f};
+    const u32x4_t one = ones<CK>();
+    const int k_lane = G::k_lane(r, g);
+    int v_lane[G::VB];
+#pragma unroll
+    for (int b = 0; b < G::VB; b++) v_lane[b] = G::v_lane(r, g, b);
     // the exponent reference, an integer that moves only when a score exceeds it by 2^SLACK: see the wide kernel below
     constexpr float SLACK = F16 ? 12.f : 64.f;
-    float e_ref = -1e30f, l_run = 0.f;
+    float e_ref = -1e30f;
     if (blk0 < blk1) {
         if constexpr (PAGED) fill_window(quot(blk0 * R16_BK, a.page));
         // (pinned: these loads have returned before the ones are issued that the compiler does not know of)
@@ -260,20 +285,18 @@ __global__ __launch_bounds__(R16_NT) void seq_attention_r16_kernel(const uint16_
         else if (G::RING > 2 && later == 1) __builtin_amdgcn_s_waitcnt(mfma::waitcnt_vm_lgkm0(2 * G::DMAS));
         else __builtin_amdgcn_s_waitcnt(mfma::waitcnt_vm_lgkm0(0));
         mfma::wave_lds_fence();
-        const char *kl = ring + slot * 2 * G::BLOCK, *vl = kl + G::BLOCK;
+        const char *kl = ring + slot * G::BLOCK, *vl = kl + G::BLOCK_K;
 
         acc_t s[2];
 #pragma unroll
         for (int t = 0; t < 2; t++) {
             s[t] = acc_t{0.f, 0.f, 0.f, 0.f};
-            const int key = 8 * (r >> 2) + 4 * t + (r & 3);
 #pragma unroll
             for (int ks = 0; ks < G::KS; ks++) {
+                const int at = k_lane + ks * G::K_STEP + t * G::K_TILE;
                 u32x4_t kf;
-                if constexpr (F8)
-                    kf = widen8<CK>(lds_get64(kl, key * G::ROW + (((2 * ks + (g >> 1)) ^ G::kswz(key)) << 4) + (g & 1) * 8));
-                else
-                    kf = lds_get(kl, key * G::ROW + (((4 * ks + g) ^ G::kswz(key)) << 4));
+                if constexpr (F8) kf = widen8<CK>(lds_get64(kl, at));
+                else kf = lds_get(kl, at);
                 Cmp::mma(kf, qf[ks], s[t]);
             }
         }
@@ -294,29 +317,24 @@ __global__ __launch_bounds__(R16_NT) void seq_attention_r16_kernel(const uint16_
             const float e_new = top > e_ref + SLACK ? ceilf(top) : e_ref;
             const float keep = __builtin_amdgcn_exp2f(e_ref - e_new);
             e_ref = e_new;
-            l_run *= keep;
 #pragma unroll
-            for (int j = 0; j < G::DT; j++)
+            for (int j = 0; j <= G::DT; j++)
 #pragma unroll
                 for (int e = 0; e < 4; e++) o[j][e] *= keep;
         }
         float p[8];
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[e], c, -e_ref));
-            l_run += p[e];  // the lane's share; the row's four lanes add up at the end
-        }
+        for (int e = 0; e < 8; e++) p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[e], c, -e_ref));
         const u32x4_t pf = {pack2<CK>(p[0], p[1]), pack2<CK>(p[2], p[3]), pack2<CK>(p[4], p[5]), pack2<CK>(p[6], p[7])};
+        Cmp::mma(one, pf, o[G::DT]);
 #pragma unroll
         for (int j = 0; j < G::DT; j++) {
+            const int at = v_lane[j % G::VB] + j / G::VB * G::V_STEP;
             u32x4_t vf;
             if constexpr (F8) {
-                const int key = 8 * g + (r >> 1);
-                vf = widen8<CK>(lds_get_tr<1>(vl, key * G::ROW + ((j ^ G::vswz(key)) << 4) + (r & 1) * 8));
+                vf = widen8<CK>(lds_get_tr<1>(vl, at));
             } else {
-                const int key = 8 * g + (r >> 2), ch = 2 * j + ((r >> 1) & 1);
-                const u32x2_t lo = lds_get_tr<2>(vl, key * G::ROW + ((ch ^ G::vswz(key)) << 4) + (r & 1) * 8);
-                const u32x2_t hi = lds_get_tr<2>(vl, (key + 4) * G::ROW + ((ch ^ G::vswz(key + 4)) << 4) + (r & 1) * 8);
+                const u32x2_t lo = lds_get_tr<2>(vl, at), hi = lds_get_tr<2>(vl, at + G::V_HALF);
                 vf = u32x4_t{lo.x, lo.y, hi.x, hi.y};
             }
             Cmp::mma(vf, pf, o[j]);
@@ -331,15 +349,13 @@ __global__ __launch_bounds__(R16_NT) void seq_attention_r16_kernel(const uint16_
     }
 
     // ---- the four wavefronts meet: per wavefront and row (reference, sum, -, -, O) ----
-    l_run += __shfl_xor(l_run, 16);
-    l_run += __shfl_xor(l_run, 32);
     __syncthreads();
     float *mg = reinterpret_cast<float *>(smem);
     {
         float *mine = mg + (wave * R16 + r) * G::LINE;
         if (g == 0) {
             mine[0] = e_ref;
-            mine[1] = l_run;
+            mine[1] = o[G::DT][0];
         }
 #pragma unroll
         for (int j = 0; j < G::DT; j++) *reinterpret_cast<f32x4_t *>(mine + 4 + 16 * j + 4 * g) = f32x4_t{o[j][0], o[j][1], o[j][2], o[j][3]};
@@ -417,12 +433,10 @@ __global__ __launch_bounds__(R16_NT) void seq_attention_r16_kernel(const uint16_
 // 4 at 64.
 template <int D> constexpr int W_TILES = D == 128 ? 3 : 4;
 constexpr int W_NT = 256, W_BK = 64, W_RING = 4, W_WINDOW = 2048;  // (the ring: stages of K and of V)
-template <int D, bool F8, bool PAGED> struct WGeom {
-    typedef R16Geom<D, F8> R;
-    static constexpr int ROW = R::ROW, CPR = R::CPR, KPI = R::KPI;   // bytes and chunks of a row, keys of an LDS-DMA instruction
-    static constexpr int BLOCK = W_BK * ROW, NI = W_BK / KPI / 4;    // instructions per block and wavefront
-    static constexpr int KS = R::KS, DT = R::DT;
-    static constexpr int V_AT = W_RING * BLOCK, TABLE_AT = 2 * V_AT;
+template <int D, bool F8, bool PAGED> struct WGeom : SeqGeom<D, F8> {
+    typedef SeqGeom<D, F8> S;
+    static constexpr int NI = 2 * S::DMAS / 4;               // LDS-DMA instructions per stage of K (of V) and wavefront
+    static constexpr int V_AT = W_RING * 2 * S::BLOCK_K, TABLE_AT = V_AT + W_RING * 2 * S::BLOCK_V;
     static constexpr int LDS = TABLE_AT + (PAGED ? W_WINDOW * 4 : 0);
 };
 
@@ -430,7 +444,6 @@ template <int CK, int D, bool PAGED, bool F8, int RT>
 __global__ __launch_bounds__(W_NT, 1) void seq_attention_wide_kernel(const uint16_t *__restrict__ Q, const char *__restrict__ K,
                                                                      const char *__restrict__ V, uint16_t *__restrict__ O, DevSeq a) {
     typedef WGeom<D, F8, PAGED> G;
-    typedef R16Geom<D, F8> R;
     typedef Compute<CK> Cmp;
     typedef typename Cmp::acc_t acc_t;
     constexpr int KS = G::KS, DT = G::DT, BM = 64 * RT;
@@ -476,14 +489,31 @@ __global__ __launch_bounds__(W_NT, 1) void seq_attention_wide_kernel(const uint1
         }
         window0 = from;
     };
+    // a lane's source within a stage of packed keys (the token stride is below 2^25 bytes: the host sees to it)
+    unsigned in_stage[2][G::NI];
+#pragma unroll
+    for (int p = 0; p < G::NI; p++) {
+        const int kk = (wave * G::NI + p) * G::KPI + lane / G::CPR;
+        in_stage[0][p] = kk * (unsigned)a.kc.token + (((lane % G::CPR) ^ G::kswz(kk & 31)) << 4);
+        in_stage[1][p] = kk * (unsigned)a.vc.token + (((lane % G::CPR) ^ G::vswz(kk & 31)) << 4);
+    }
     auto issue = [&](int stage, bool is_v) __attribute__((always_inline)) {
-        const int at = (is_v ? G::V_AT : 0) + (stage & (W_RING - 1)) * G::BLOCK;
+        const PagedSide &side = is_v ? a.vc : a.kc;
+        const char *base = is_v ? vbase : kbase;
+        const unsigned padded = is_v ? G::PADDED_V : G::PADDED_K;
+        // (a stage is two blocks of 32 keys, the ring eight)
+        const unsigned to = lds0 + (is_v ? G::V_AT : 0) + (stage & (W_RING - 1)) * 2 * (is_v ? G::BLOCK_V : G::BLOCK_K) + wave * G::NI * padded;
+        if (!PAGED && (stage + 1) * W_BK <= keys) {
+            const char *from = base + (long)(k0 + stage * W_BK) * side.token;
+#pragma unroll
+            for (int p = 0; p < G::NI; p++) mfma::dma16_sbase(from, in_stage[is_v][p], __builtin_amdgcn_readfirstlane(to + p * padded));
+            return;
+        }
 #pragma unroll
         for (int p = 0; p < G::NI; p++) {
-            const int i = wave * G::NI + p, kk = i * G::KPI + lane / G::CPR;
+            const int kk = (wave * G::NI + p) * G::KPI + lane / G::CPR;
             int key = stage * W_BK + kk;
             key = key < keys ? key : keys - 1;  // behind the last key: that one again, masked below
-            const PagedSide &side = is_v ? a.vc : a.kc;
             long off;
             if constexpr (PAGED) {
                 const int col = quot(key, a.page);
@@ -491,48 +521,41 @@ __global__ __launch_bounds__(W_NT, 1) void seq_attention_wide_kernel(const uint1
             } else {
                 off = (k0 + key) * side.token;
             }
-            const int chunk = (lane % G::CPR) ^ (is_v ? R::vswz(kk & 31) : R::kswz(kk & 31));
-            mfma::dma16_raw((is_v ? vbase : kbase) + off + (chunk << 4), __builtin_amdgcn_readfirstlane(lds0 + at + i * 1024));
+            const int chunk = (lane % G::CPR) ^ (is_v ? G::vswz(kk & 31) : G::kswz(kk & 31));
+            mfma::dma16_raw(base + off + (chunk << 4), __builtin_amdgcn_readfirstlane(to + p * padded));
         }
     };
 
-    acc_t o[RT][DT];
-    float e_ref[RT], l_run[RT], top[RT];  // exponent reference, the lane's share of the row sum, the lane's largest new score
+    acc_t o[RT][DT + 1];           // the last tile: the row sums
+    float e_ref[RT], top[RT];      // exponent reference, the lane's largest new score
+    const u32x4_t one = ones<CK>();
 #pragma unroll
     for (int x = 0; x < RT; x++) {
 #pragma unroll
-        for (int j = 0; j < DT; j++) o[x][j] = acc_t{0.f, 0.f, 0.f, 0.f};
+        for (int j = 0; j <= DT; j++) o[x][j] = acc_t{0.f, 0.f, 0.f, 0.f};
         e_ref[x] = -1e30f;  // no key yet
-        l_run[x] = 0.f;
     }
 
-    // fragments.  K fragment q = 2 ks + t: 16 keys of tile t, 32 of the head dim (8-bit: raw bytes).  V fragment j: 32 keys, 16 of
-    // the head dim, through VR transpose reads
-    constexpr int KF = 2 * KS, VR = F8 ? 1 : 2;
-    typedef typename std::conditional<F8, u32x2_t, u32x4_t>::type raw_t;
+    constexpr int KF = G::KF, VR = G::VR;
+    typedef typename std::conditional<F8, u32x2_t, u32x4_t>::type raw_t;  // (8-bit: raw bytes, widened at their use)
     raw_t kf[KF];
     u32x2_t vf[DT * VR];
-    int k_at[2];
+    const int k_lane = G::k_lane(r, g);
+    int v_lane[G::VB];
 #pragma unroll
-    for (int t = 0; t < 2; t++) {
-        const int key = 8 * (r >> 2) + 4 * t + (r & 3);
-        k_at[t] = key * G::ROW + (((F8 ? g >> 1 : g) ^ R::kswz(key)) << 4) + (F8 ? (g & 1) * 8 : 0);
-    }
-    const int v_key = 8 * g + (F8 ? r >> 1 : r >> 2);
-    const int v_at = G::V_AT + v_key * G::ROW + (((F8 ? 0 : (r >> 1) & 1) ^ R::vswz(v_key)) << 4) + (r & 1) * 8;
-    const int v_at4 = G::V_AT + (v_key + 4) * G::ROW + ((((r >> 1) & 1) ^ R::vswz(v_key + 4)) << 4) + (r & 1) * 8;  // 16-bit: keys + 4
-    auto read_k = [&](int q, int at) __attribute__((always_inline)) {  // (the chunk index is XORed, so a fragment's distance along the head dim is one on the address)
-        const int ks = q >> 1, t = q & 1;
-        if constexpr (F8) kf[q] = lds_get64(smem + at, k_at[t] ^ (ks << 5));
-        else kf[q] = lds_get(smem + at, k_at[t] ^ (ks << 6));
+    for (int b2 = 0; b2 < G::VB; b2++) v_lane[b2] = G::V_AT + G::v_lane(r, g, b2);
+    auto read_k = [&](int q, int at) __attribute__((always_inline)) {
+        const int from = k_lane + at + (q >> 1) * G::K_STEP + (q & 1) * G::K_TILE;
+        if constexpr (F8) kf[q] = lds_get64(smem, from);
+        else kf[q] = lds_get(smem, from);
     };
     auto k_operand = [&](int q) __attribute__((always_inline)) -> u32x4_t {
         if constexpr (F8) return widen8<CK>(kf[q]);
         else return kf[q];
     };
     auto read_v = [&](int q, int at) __attribute__((always_inline)) {
-        if constexpr (F8) vf[q] = lds_get_tr<1>(smem + at, v_at ^ (q << 4));
-        else vf[q] = lds_get_tr<2>(smem + at, ((q & 1) ? v_at4 : v_at) ^ ((q >> 1) << 5));
+        const int j = q / VR, from = v_lane[j % G::VB] + at + j / G::VB * G::V_STEP + q % VR * G::V_HALF;
+        vf[q] = lds_get_tr<F8 ? 1 : 2>(smem, from);
     };
     auto v_operand = [&](int j) __attribute__((always_inline)) -> u32x4_t {
         if constexpr (F8) return widen8<CK>(vf[j]);
@@ -568,9 +591,8 @@ __global__ __launch_bounds__(W_NT, 1) void seq_attention_wide_kernel(const uint1
             const float e_new = most > e_ref[x] + SLACK ? ceilf(most) : e_ref[x];
             const float f = __builtin_amdgcn_exp2f(e_ref[x] - e_new);
             e_ref[x] = e_new;
-            l_run[x] *= f;
 #pragma unroll
-            for (int j = 0; j < DT; j++) mfma::scale4_acc(o[x][j], f);
+            for (int j = 0; j <= DT; j++) mfma::scale4_acc(o[x][j], f);
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 const uint32_t pw = pc[x][i];
@@ -592,8 +614,6 @@ __global__ __launch_bounds__(W_NT, 1) void seq_attention_wide_kernel(const uint1
     auto exponential = [&](const acc_t (&sc)[RT][2], u32x4_t (&pc)[RT], int t) __attribute__((always_inline)) {
         const int x = t >> 3, e = t & 7;
         const float v = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[x][e >> 2][e & 3], c, -e_ref[x]));
-        l_run[x] += v;
-        mfma::pin_vector(l_run[x]);
         if (e & 1) {
             pc[x][e >> 1] = pack2<CK>(pair, v);
             uint32_t w = pc[x][e >> 1];
@@ -601,6 +621,7 @@ __global__ __launch_bounds__(W_NT, 1) void seq_attention_wide_kernel(const uint1
             pc[x][e >> 1] = w;
         } else {
             pair = v;
+            mfma::pin_vector(pair);
         }
     };
     constexpr int NQ = KF * RT, NP = DT * RT, EL = 8 * RT, EVERY = (NQ + NP) / EL;
@@ -629,6 +650,7 @@ __global__ __launch_bounds__(W_NT, 1) void seq_attention_wide_kernel(const uint1
                 else mfma::mfma16_next<F16, F8>(k_operand(q), qf[x][q >> 1], sn[x][q & 1]);
             } else {
                 Cmp::mma(v_operand(u / RT), pp[u % RT], o[u % RT][u / RT]);
+                if (u >= NP - RT) Cmp::mma(one, pp[u % RT], o[u % RT][DT]);
             }
             if (t % EVERY == 0) exponential(sc, pc, t / EVERY);
             const int soon = t + AHEAD;  // the instruction whose fragment is read now, if it is the first to use it
@@ -663,12 +685,15 @@ __global__ __launch_bounds__(W_NT, 1) void seq_attention_wide_kernel(const uint1
             __builtin_amdgcn_sched_barrier(0);
         }
     };
-    // where K or V of step i lies in its ring
-    auto block_of = [&](int i) __attribute__((always_inline)) { return (i >> 1 & (W_RING - 1)) * G::BLOCK + (i & 1) * 32 * G::ROW; };
+    // where K and V of step i lie in their rings
+    auto k_of = [&](int i) __attribute__((always_inline)) { return (i & (2 * W_RING - 1)) * G::BLOCK_K; };
+    auto v_of = [&](int i) __attribute__((always_inline)) { return (i & (2 * W_RING - 1)) * G::BLOCK_V; };
     // the same step one piece after the other with few registers, for what is masked, first or last; sc: scores of step i, replaced by
     // those of i + 1; pc: P of step i - 1, replaced by that of i
     auto times_v = [&](int i, const u32x4_t (&pp)[RT]) __attribute__((always_inline)) {
-        const int at = block_of(i);
+        const int at = v_of(i);
+#pragma unroll
+        for (int x = 0; x < RT; x++) Cmp::mma(one, pp[x], o[x][DT]);
 #pragma unroll
         for (int j = 0; j < DT; j++) {
 #pragma unroll
@@ -683,7 +708,7 @@ __global__ __launch_bounds__(W_NT, 1) void seq_attention_wide_kernel(const uint1
         if (i >= 0)
 #pragma unroll
             for (int t = 0; t < EL; t++) exponential(sc, pc, t);
-        const int at = block_of(i + 1);
+        const int at = k_of(i + 1);
 #pragma unroll
         for (int q = 0; q < KF; q++) {
             read_k(q, at);
@@ -704,8 +729,8 @@ __global__ __launch_bounds__(W_NT, 1) void seq_attention_wide_kernel(const uint1
             __syncthreads();
         }
         // step 0 multiplies a P of zeros by what lies where V of the step before it would: zeros too
-        for (int i = tid; i < 32 * G::ROW / 16; i += W_NT)
-            *reinterpret_cast<u32x4_t *>(smem + G::V_AT + (W_RING - 1) * G::BLOCK + 32 * G::ROW + i * 16) = u32x4_t{0, 0, 0, 0};
+        for (int i = tid; i < G::BLOCK_V / 16; i += W_NT)
+            *reinterpret_cast<u32x4_t *>(smem + G::V_AT + (2 * W_RING - 1) * G::BLOCK_V + i * 16) = u32x4_t{0, 0, 0, 0};
         issue(0, false);
         if (stages > 1) issue(1, false);
         issue(0, true);
@@ -750,13 +775,13 @@ __global__ __launch_bounds__(W_NT, 1) void seq_attention_wide_kernel(const uint1
             if (!(i & 1) && (2 * st + 3) * 32 <= all_open) {
                 acc_t sn[RT][2];     // scores of the odd steps, those of the even ones in sc
                 u32x4_t pn[RT];      // P of the even steps, that of the odd ones in pc
-                first_fragments(block_of(2 * st + 1));
+                first_fragments(k_of(2 * st + 1));
                 bool half = false;
                 do {
                     begin_stage();
-                    step(sc, sn, pc, pn, block_of(2 * st - 1), block_of(2 * st + 1), block_of(2 * st + 2));
+                    step(sc, sn, pc, pn, v_of(2 * st - 1), k_of(2 * st + 1), k_of(2 * st + 2));
                     if (some_exceed()) { half = true; break; }
-                    step(sn, sc, pn, pc, block_of(2 * st), block_of(2 * st + 2), block_of(2 * st + 3));
+                    step(sn, sc, pn, pc, v_of(2 * st), k_of(2 * st + 2), k_of(2 * st + 3));
                     st++;
                 } while (!some_exceed() && (2 * st + 3) * 32 <= all_open);
                 i = 2 * st + (half ? 1 : 0);
@@ -783,9 +808,7 @@ __global__ __launch_bounds__(W_NT, 1) void seq_attention_wide_kernel(const uint1
 #pragma unroll
     for (int x = 0; x < RT; x++) {
         const int row = wrow0 + 16 * x + r;
-        float l = l_run[x];
-        l += __shfl_xor(l, 16);
-        l += __shfl_xor(l, 32);
+        const float l = o[x][DT][0];
         const float inv = l == 0.f ? 0.f : (F8 ? a.v_scale[kvh] : 1.f) / l;  // a row without keys is zero
         if (row >= rows) continue;
         const int tok = quot(row, a.by_group), head = kvh * a.group + row - tok * a.group;
@@ -842,11 +865,13 @@ int launch_seq_attention(hodu_rocm_ctx *ctx, int dtype, int cache_dtype, const v
     auto by_form = [&](auto ck, auto d, auto paged, auto f8_) -> int {
         constexpr int CK = decltype(ck)::value, D = decltype(d)::value;
         constexpr bool PAGED = decltype(paged)::value, F8 = decltype(f8_)::value;
+        // packed keys of the wide kernels: a stage's keys by a 32-bit offset
+        const bool near = PAGED || (a.kc.token < (1L << 25) && a.vc.token < (1L << 25));
         const int pin = ctx->force_tile;  // testing hook: 50 tiles of 16 rows, 51 of 128, 52 of 192 or 256
-        if (pin == 52 || (pin < 50 && avg_rows >= 192))
+        if (near && (pin == 52 || (pin < 50 && avg_rows >= 192)))
             return launch(seq_attention_wide_kernel<CK, D, PAGED, F8, W_TILES<D>>, 64 * W_TILES<D>, W_NT, WGeom<D, F8, PAGED>::LDS,
                           !PAGED ? "attention_varlen_wide" : F8 ? "attention_paged_wide_f8" : "attention_paged_wide");
-        if (pin == 51 || (pin < 50 && avg_rows >= 48))
+        if (near && (pin == 51 || (pin < 50 && avg_rows >= 48)))
             return launch(seq_attention_wide_kernel<CK, D, PAGED, F8, 2>, 128, W_NT, WGeom<D, F8, PAGED>::LDS,
                           !PAGED ? "attention_varlen_wide128" : F8 ? "attention_paged_wide128_f8" : "attention_paged_wide128");
         // Few tiles over long contexts: the keys are cut across workgroups, to about eight per compute unit (they differ in

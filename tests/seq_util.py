@@ -88,10 +88,11 @@ def allowed(dt, o, a, size, inv, m, vmax, d):
         exponential that is a relative error of P, and of l: 2 (D + 2) e size; base-2 exponential, its argument's
         fused multiply-add (|argument| e) and the rescalings 8 e + size e, twice
       * sums over the keys in f32: (m + 8) e a
+      * the row sum is taken over the rounded P: off by u of itself at most, u |o|
       * the result is rounded once: u |o|, in f16 at least 2^-25"""
     u, e = HALF_STEP[dt], 2.0 ** -24
     rel = u + 2 * ((d + 2) * e * size + 8 * e + 2 * size * e) + (m + 8) * e
-    tol = a * rel[..., None] + np.abs(o) * u
+    tol = a * rel[..., None] + 2 * np.abs(o) * u
     if dt == "f16":
         tol = tol + (m * 2.0 ** -25 * inv * vmax)[..., None] + 2.0 ** -25
     return tol * (1 + 2 * u) + 1e-30
