@@ -626,17 +626,19 @@ __global__ __launch_bounds__(W_NT, 1) void seq_attention_wide_kernel(const uint1
     };
     constexpr int NQ = KF * RT, NP = DT * RT, EL = 8 * RT, EVERY = (NQ + NP) / EL;
     static_assert(EVERY * EL == NQ + NP, "the exponentials spread evenly over the matrix instructions");
-    // Step i of a wavefront whose rows attend all of it and of the next: scores of i + 1 (into sn) and the lane's largest of them,
-    // exponentials of i (sc, into pc), P V of i - 1 (pp).  v_block: where V of step i - 1 lies, k_block: K of step i + 1, k_next: of step
-    // i + 2.  A fragment is read AHEAD chunks (16 cycles each) before its first use: the first ones of a step in the step before.
+    // where K and V of step i lie in their rings
+    auto k_of = [&](int i) __attribute__((always_inline)) { return (i & (2 * W_RING - 1)) * G::BLOCK_K; };
+    auto v_of = [&](int i) __attribute__((always_inline)) { return (i & (2 * W_RING - 1)) * G::BLOCK_V; };
+    // Step i: scores of i + 1 (into sn) and the lane's largest of them, exponentials of i (sc, into pc), P V of i - 1 (pp).  A fragment is read AHEAD chunks (16 cycles each) before its first use: the first ones of a step in the step before.
     constexpr int AHEAD = NQ < 10 ? NQ : 10;
     auto first_fragments = [&](int k_block) __attribute__((always_inline)) {
 #pragma unroll
         for (int q = 0; q < KF; q++)
             if (q * RT < AHEAD) read_k(q, k_block);
     };
-    auto step = [&](const acc_t (&sc)[RT][2], acc_t (&sn)[RT][2], const u32x4_t (&pp)[RT], u32x4_t (&pc)[RT], int v_block, int k_block,
-                    int k_next) __attribute__((always_inline)) {
+    // masked: some row may not attend all of step i + 1
+    auto step = [&](auto masked, int i, const acc_t (&sc)[RT][2], acc_t (&sn)[RT][2], const u32x4_t (&pp)[RT], u32x4_t (&pc)[RT]) __attribute__((always_inline)) {
+        const int v_block = v_of(i - 1), k_block = k_of(i + 1), k_next = k_of(i + 2);
         constexpr int FROM = NP / 4, MPC = (EL + NP - FROM - 1) / (NP - FROM);
         static_assert(FROM >= 2 && AHEAD <= NP, "");
 #pragma unroll
@@ -672,6 +674,7 @@ __global__ __launch_bounds__(W_NT, 1) void seq_attention_wide_kernel(const uint1
                     mfma::pin_vector(sn[x][0]);
                     mfma::pin_vector(sn[x][1]);
                 }
+                if constexpr (decltype(masked)::value) mask(sn, i + 1);
             }
             if (u >= FROM) {  // the lane's largest new score
 #pragma unroll
@@ -685,10 +688,7 @@ __global__ __launch_bounds__(W_NT, 1) void seq_attention_wide_kernel(const uint1
             __builtin_amdgcn_sched_barrier(0);
         }
     };
-    // where K and V of step i lie in their rings
-    auto k_of = [&](int i) __attribute__((always_inline)) { return (i & (2 * W_RING - 1)) * G::BLOCK_K; };
-    auto v_of = [&](int i) __attribute__((always_inline)) { return (i & (2 * W_RING - 1)) * G::BLOCK_V; };
-    // the same step one piece after the other with few registers, for what is masked, first or last; sc: scores of step i, replaced by
+    // the same step one piece after the other with few registers, for the first scores and behind a reference that moved; sc: scores of step i, replaced by
     // those of i + 1; pc: P of step i - 1, replaced by that of i
     auto times_v = [&](int i, const u32x4_t (&pp)[RT]) __attribute__((always_inline)) {
         const int at = v_of(i);
@@ -761,9 +761,9 @@ __global__ __launch_bounds__(W_NT, 1) void seq_attention_wide_kernel(const uint1
             if (st + 3 < stages) issue(st + 3, false);
             if (st + 2 < stages) issue(st + 2, true);
         };
-        // The stages whose scores are all open run in a loop that holds nothing but the two steps: a rarely taken block that
-        // touches O or P and joins the loop again makes the allocator spill inside it.  Whatever else there is -- an edge, a
-        // reference to move -- leaves the loop, takes slow steps, and comes back.
+        // Two loops, one for stages whose scores are all open and one that masks, hold nothing but the two steps: a rarely taken
+        // block that touches O or P and joins the loop again makes the allocator spill inside it.  A reference to move leaves the
+        // loop, takes a slow step if that was in the middle of a stage, and comes back.
         acc_t sc[RT][2];
         u32x4_t pc[RT];
 #pragma unroll
@@ -772,18 +772,28 @@ __global__ __launch_bounds__(W_NT, 1) void seq_attention_wide_kernel(const uint1
         if (some_exceed()) move_references(pc);
         int i = 0;  // the step in front of us; i = 2 st + 1: in the middle of a stage
         while (st < stages) {
-            if (!(i & 1) && (2 * st + 3) * 32 <= all_open) {
+            if (!(i & 1) && i <= steps) {
                 acc_t sn[RT][2];     // scores of the odd steps, those of the even ones in sc
                 u32x4_t pn[RT];      // P of the even steps, that of the odd ones in pc
                 first_fragments(k_of(2 * st + 1));
                 bool half = false;
-                do {
-                    begin_stage();
-                    step(sc, sn, pc, pn, v_of(2 * st - 1), k_of(2 * st + 1), k_of(2 * st + 2));
-                    if (some_exceed()) { half = true; break; }
-                    step(sn, sc, pn, pc, v_of(2 * st), k_of(2 * st + 2), k_of(2 * st + 3));
-                    st++;
-                } while (!some_exceed() && (2 * st + 3) * 32 <= all_open);
+                if ((2 * st + 3) * 32 <= all_open) {
+                    do {
+                        begin_stage();
+                        step(std::false_type(), 2 * st, sc, sn, pc, pn);
+                        if (some_exceed()) { half = true; break; }
+                        step(std::false_type(), 2 * st + 1, sn, sc, pn, pc);
+                        st++;
+                    } while (!some_exceed() && (2 * st + 3) * 32 <= all_open);
+                } else {
+                    do {
+                        begin_stage();
+                        step(std::true_type(), 2 * st, sc, sn, pc, pn);
+                        if (some_exceed()) { half = true; break; }
+                        step(std::true_type(), 2 * st + 1, sn, sc, pn, pc);
+                        st++;
+                    } while (!some_exceed() && 2 * st <= steps && st < stages);
+                }
                 i = 2 * st + (half ? 1 : 0);
                 if (half) {
 #pragma unroll
