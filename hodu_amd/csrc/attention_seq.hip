@@ -40,52 +40,69 @@ struct DevSeq {
     int causal;
 };
 
-__device__ __forceinline__ int quot(int n, const FixedDiv &f) { return (int)(((unsigned long long)(unsigned)n * f.mul) >> f.sh); }
+__device__ __forceinline__ int quot(int n, const FixedDiv &f) { return fixed_quotient(n, f); }
 
-// what lane `from` of the wavefront holds
-__device__ __forceinline__ int from_lane(int v, int from) { return __builtin_amdgcn_ds_bpermute(from << 2, v); }
+// inclusive running sum over the wavefront's lanes (each step one instruction: shifts by 1, 2, 4, 8 within rows of 16 lanes, then
+// each row's last lane to the next row, then lane 31 to the upper half)
+__device__ __forceinline__ int running_sum64(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
+    return v;
+}
 
 // The sequence and first row of tile `tile` of `rows` rows (found by the whole wavefront, the same in all lanes); false
-// past the last tile.  n: the sequence's tokens, q0: its first one; m: its keys and, packed, k0: where they begin
+// past the last tile.  n: the sequence's tokens, q0: its first one; m: its keys and, packed, k0: where they begin.
+// Every workgroup searches for itself, four sequences a lane, 256 at a step (a step is a trip to memory; a serving batch is one or two).
 struct SeqTile {
     int b, row0, q0, n, k0, m;
 };
 template <int ROWS, bool PAGED> __device__ __forceinline__ bool find_tile(const DevSeq &a, int tile, SeqTile &f) {
     const int lane = threadIdx.x & 63;
     int before = 0;
-    for (int base = 0; base < a.batch; base += 64) {
-        const int s = base + lane;
-        int lo = 0, len = 0, k0 = 0, m = 0;
-        if (s < a.batch) {
-            const int qa = a.q_offsets[s], qb = a.q_offsets[s + 1];
-            int ka = 0, kb;
-            if constexpr (PAGED) kb = a.lens[s];
-            else ka = a.k_offsets[s], kb = a.k_offsets[s + 1];
-            const int hi = qb < a.q_tokens ? qb : a.q_tokens;
-            lo = qa > 0 ? qa : 0;
-            len = hi > lo ? hi - lo : 0;
-            const int k_most = PAGED ? a.width * a.page.d : a.k_tokens, k_hi = kb < k_most ? kb : k_most;
-            k0 = ka > 0 ? ka : 0;
-            m = k_hi > k0 ? k_hi - k0 : 0;
-        }
-        const int tiles = (int)(((long)len * a.group + ROWS - 1) / ROWS);
-        int sum = tiles;  // inclusive over the lanes
+    for (int base = 0; base < a.batch; base += 256) {
+        const int s0 = base + 4 * lane;
+        int q[5], k[5], tiles[4], lo[4], len[4], own = 0;
 #pragma unroll
-        for (int step = 1; step < 64; step *= 2) {
-            const int up = from_lane(sum, lane >= step ? lane - step : lane);
-            sum += lane >= step ? up : 0;
+        for (int i = 0; i < 5; i++) {
+            const int s = s0 + i < a.batch ? s0 + i : a.batch;  // (there are batch + 1 offsets)
+            q[i] = a.q_offsets[s];
+            if constexpr (PAGED) k[i] = a.lens[s < a.batch ? s : a.batch - 1];
+            else k[i] = a.k_offsets[s];
         }
-        const int all = from_lane(sum, 63);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int hi = q[i + 1] < a.q_tokens ? q[i + 1] : a.q_tokens;
+            lo[i] = q[i] > 0 ? q[i] : 0;
+            len[i] = s0 + i < a.batch && hi > lo[i] ? hi - lo[i] : 0;
+            tiles[i] = (int)(((long)len[i] * a.group + ROWS - 1) / ROWS);
+            own += tiles[i];
+        }
+        const int sum = running_sum64(own), all = __builtin_amdgcn_readlane(sum, 63);
         if (tile < before + all) {
             const unsigned long long past = __builtin_amdgcn_ballot_w64(before + sum > tile);
             const int at = __builtin_ctzll(past);
-            const int first = before + from_lane(sum, at) - from_lane(tiles, at);
-            f.b = __builtin_amdgcn_readfirstlane(base + at);
-            f.q0 = __builtin_amdgcn_readfirstlane(from_lane(lo, at));
-            f.n = __builtin_amdgcn_readfirstlane(from_lane(len, at));
-            f.k0 = __builtin_amdgcn_readfirstlane(from_lane(k0, at));
-            f.m = __builtin_amdgcn_readfirstlane(from_lane(m, at));
-            f.row0 = __builtin_amdgcn_readfirstlane((tile - first) * ROWS);
+            int left = tile - (before + __builtin_amdgcn_readlane(sum - own, at)), i = 0, t[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) t[j] = __builtin_amdgcn_readlane(tiles[j], at);
+#pragma unroll
+            for (int j = 0; j < 3; j++)
+                if (i == j && left >= t[j]) left -= t[j], i = j + 1;
+            f.b = base + 4 * at + i;
+            f.row0 = left * ROWS;
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (i == j) {
+                    f.q0 = __builtin_amdgcn_readlane(lo[j], at);
+                    f.n = __builtin_amdgcn_readlane(len[j], at);
+                    const int ka = PAGED ? 0 : __builtin_amdgcn_readlane(k[j], at), kb = __builtin_amdgcn_readlane(k[PAGED ? j : j + 1], at);
+                    const int most = PAGED ? a.width * a.page.d : a.k_tokens, k_hi = kb < most ? kb : most;
+                    f.k0 = ka > 0 ? ka : 0;
+                    f.m = k_hi > f.k0 ? k_hi - f.k0 : 0;
+                }
             // (offsets that do not ascend can make the count above wrap; a tile outside its sequence is no tile)
             return f.row0 >= 0 && f.row0 < (long)f.n * a.group;
         }
@@ -497,6 +514,20 @@ __global__ __launch_bounds__(W_NT, 1) void seq_attention_wide_kernel(const uint1
         in_stage[0][p] = kk * (unsigned)a.kc.token + (((lane % G::CPR) ^ G::kswz(kk & 31)) << 4);
         in_stage[1][p] = kk * (unsigned)a.vc.token + (((lane % G::CPR) ^ G::vswz(kk & 31)) << 4);
     }
+    // The same of a paged cache: page and token within it of the lane's key of each instruction.  K is loaded a stage ahead of V, so a
+    // key is looked up once, in the stage before its K is issued (between the matrix instructions), and what K used V uses next.
+    [[maybe_unused]] int k_page[G::NI], k_in[G::NI], v_page[G::NI], v_in[G::NI];
+    auto look_up = [&](int stage, int p) __attribute__((always_inline)) {
+        int key = stage * W_BK + (wave * G::NI + p) * G::KPI + lane / G::CPR;
+        key = key < keys ? key : keys - 1;  // behind the last key: that one again, masked below
+        const int col = quot(key, a.page);
+        k_page[p] = window[col - window0];
+        k_in[p] = key - col * a.page.d;
+    };
+    auto pass_on = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int p = 0; p < G::NI; p++) v_page[p] = k_page[p], v_in[p] = k_in[p];
+    };
     auto issue = [&](int stage, bool is_v) __attribute__((always_inline)) {
         const PagedSide &side = is_v ? a.vc : a.kc;
         const char *base = is_v ? vbase : kbase;
@@ -512,13 +543,12 @@ __global__ __launch_bounds__(W_NT, 1) void seq_attention_wide_kernel(const uint1
 #pragma unroll
         for (int p = 0; p < G::NI; p++) {
             const int kk = (wave * G::NI + p) * G::KPI + lane / G::CPR;
-            int key = stage * W_BK + kk;
-            key = key < keys ? key : keys - 1;  // behind the last key: that one again, masked below
             long off;
             if constexpr (PAGED) {
-                const int col = quot(key, a.page);
-                off = window[col - window0] * side.page + (key - col * a.page.d) * side.token;
+                off = (is_v ? v_page[p] : k_page[p]) * side.page + (is_v ? v_in[p] : k_in[p]) * side.token;
             } else {
+                int key = stage * W_BK + kk;
+                key = key < keys ? key : keys - 1;  // behind the last key: that one again, masked below
                 off = (k0 + key) * side.token;
             }
             const int chunk = (lane % G::CPR) ^ (is_v ? G::vswz(kk & 31) : G::kswz(kk & 31));
@@ -603,6 +633,15 @@ __global__ __launch_bounds__(W_NT, 1) void seq_attention_wide_kernel(const uint1
         mfma::mfma_results_settle();
         __builtin_amdgcn_sched_barrier(0);
     };
+    // the first ones: there is nothing to rescale yet
+    auto set_references = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int x = 0; x < RT; x++) {
+            float most = __builtin_fmaxf(top[x], __shfl_xor(top[x], 16));
+            most = c * __builtin_fmaxf(most, __shfl_xor(most, 32));
+            if (most > e_ref[x] + SLACK) e_ref[x] = ceilf(most);
+        }
+    };
     auto some_exceed = [&]() __attribute__((always_inline)) {
         bool up = false;
 #pragma unroll
@@ -637,7 +676,7 @@ __global__ __launch_bounds__(W_NT, 1) void seq_attention_wide_kernel(const uint1
             if (q * RT < AHEAD) read_k(q, k_block);
     };
     // masked: some row may not attend all of step i + 1
-    auto step = [&](auto masked, int i, const acc_t (&sc)[RT][2], acc_t (&sn)[RT][2], const u32x4_t (&pp)[RT], u32x4_t (&pc)[RT]) __attribute__((always_inline)) {
+    auto step = [&](auto masked, auto second, int i, const acc_t (&sc)[RT][2], acc_t (&sn)[RT][2], const u32x4_t (&pp)[RT], u32x4_t (&pc)[RT]) __attribute__((always_inline)) {
         const int v_block = v_of(i - 1), k_block = k_of(i + 1), k_next = k_of(i + 2);
         constexpr int FROM = NP / 4, MPC = (EL + NP - FROM - 1) / (NP - FROM);
         static_assert(FROM >= 2 && AHEAD <= NP, "");
@@ -665,6 +704,9 @@ __global__ __launch_bounds__(W_NT, 1) void seq_attention_wide_kernel(const uint1
             } else if ((soon - NQ - NP) % RT == 0) {
                 read_k((soon - NQ - NP) / RT, k_next);
             }
+            // (in the second step of a stage: the keys whose K the next stage issues)
+            if constexpr (PAGED && decltype(second)::value)
+                if (t % 8 == 1 && t / 8 < G::NI) look_up((i >> 1) + 4, t / 8);
             if (u == FROM) {
                 // Here the scores become values that anything but a matrix instruction may use: the compiler, which knows nothing
                 // of the wait states behind an instruction it has not chosen, copies them for the loop's exits.  (The last one of
@@ -695,13 +737,11 @@ __global__ __launch_bounds__(W_NT, 1) void seq_attention_wide_kernel(const uint1
 #pragma unroll
         for (int x = 0; x < RT; x++) Cmp::mma(one, pp[x], o[x][DT]);
 #pragma unroll
-        for (int j = 0; j < DT; j++) {
+        for (int q = 0; q < DT * VR; q++) read_v(q, at);
 #pragma unroll
-            for (int q = 0; q < VR; q++) read_v(j * VR + q, at);
+        for (int j = 0; j < DT; j++)
 #pragma unroll
             for (int x = 0; x < RT; x++) Cmp::mma(v_operand(j), pp[x], o[x][j]);
-            __builtin_amdgcn_sched_barrier(0);
-        }
     };
     auto slow_step = [&](int i, acc_t (&sc)[RT][2], u32x4_t (&pc)[RT]) __attribute__((always_inline)) {
         if (i > 0) times_v(i - 1, pc);
@@ -710,15 +750,14 @@ __global__ __launch_bounds__(W_NT, 1) void seq_attention_wide_kernel(const uint1
             for (int t = 0; t < EL; t++) exponential(sc, pc, t);
         const int at = k_of(i + 1);
 #pragma unroll
-        for (int q = 0; q < KF; q++) {
-            read_k(q, at);
+        for (int q = 0; q < KF; q++) read_k(q, at);
+#pragma unroll
+        for (int q = 0; q < KF; q++)
 #pragma unroll
             for (int x = 0; x < RT; x++) {
                 if (q < 2) sc[x][q & 1] = acc_t{0.f, 0.f, 0.f, 0.f};
                 Cmp::mma(k_operand(q), qf[x][q >> 1], sc[x][q & 1]);
             }
-            __builtin_amdgcn_sched_barrier(0);
-        }
         if ((i + 2) * 32 > all_open) mask(sc, i + 1);  // some row does not attend all of step i + 1
         largest(sc);
     };
@@ -731,11 +770,18 @@ __global__ __launch_bounds__(W_NT, 1) void seq_attention_wide_kernel(const uint1
         // step 0 multiplies a P of zeros by what lies where V of the step before it would: zeros too
         for (int i = tid; i < G::BLOCK_V / 16; i += W_NT)
             *reinterpret_cast<u32x4_t *>(smem + G::V_AT + (2 * W_RING - 1) * G::BLOCK_V + i * 16) = u32x4_t{0, 0, 0, 0};
-        issue(0, false);
-        if (stages > 1) issue(1, false);
-        issue(0, true);
-        if (stages > 2) issue(2, false);
-        if (stages > 1) issue(1, true);
+#pragma unroll
+        for (int ahead = 0; ahead < 3; ahead++) {
+            if constexpr (PAGED)
+#pragma unroll
+                for (int p = 0; p < G::NI; p++) look_up(ahead, p);
+            if (ahead < stages) issue(ahead, false);
+            if constexpr (PAGED) pass_on();
+            if (ahead < 2 && ahead < stages) issue(ahead, true);
+        }
+        if constexpr (PAGED)
+#pragma unroll
+            for (int p = 0; p < G::NI; p++) look_up(3, p);
         __builtin_amdgcn_s_waitcnt(mfma::waitcnt_vm_lgkm0(0));
         // (pinned, so that the compiler knows on every path into the loop that these loads have returned)
 #pragma unroll
@@ -750,16 +796,18 @@ __global__ __launch_bounds__(W_NT, 1) void seq_attention_wide_kernel(const uint1
             if (st > 0 && st + 2 < stages) __builtin_amdgcn_s_waitcnt(mfma::waitcnt_vm_lgkm0(2 * G::NI));
             else __builtin_amdgcn_s_waitcnt(mfma::waitcnt_vm_lgkm0(0));
             __syncthreads();
+            if (st + 2 < stages) issue(st + 2, true);
+            if (st + 3 < stages) issue(st + 3, false);
             if constexpr (PAGED) {
-                // the table columns of the keys that are to be loaded: V of stage st + 2 (the least) .. K of stage st + 3
-                const int hi = (st + 4) * W_BK - 1 < keys ? (st + 4) * W_BK - 1 : keys - 1;
-                if (st + 2 < stages && quot(hi, a.page) - window0 >= W_WINDOW) {
-                    fill_window(quot((st + 2) * W_BK, a.page));
+                pass_on();
+                // the table columns of the keys that are looked up in this stage, K of stage st + 4
+                const int hi = (st + 5) * W_BK - 1 < keys ? (st + 5) * W_BK - 1 : keys - 1;
+                if (st + 4 < stages && quot(hi, a.page) - window0 >= W_WINDOW) {
+                    __syncthreads();  // (everybody has looked up what the window held)
+                    fill_window(quot((st + 4) * W_BK, a.page));
                     __syncthreads();
                 }
             }
-            if (st + 3 < stages) issue(st + 3, false);
-            if (st + 2 < stages) issue(st + 2, true);
         };
         // Two loops, one for stages whose scores are all open and one that masks, hold nothing but the two steps: a rarely taken
         // block that touches O or P and joins the loop again makes the allocator spill inside it.  A reference to move leaves the
@@ -769,7 +817,7 @@ __global__ __launch_bounds__(W_NT, 1) void seq_attention_wide_kernel(const uint1
 #pragma unroll
         for (int x = 0; x < RT; x++) pc[x] = u32x4_t{0, 0, 0, 0};
         slow_step(-1, sc, pc);
-        if (some_exceed()) move_references(pc);
+        set_references();
         int i = 0;  // the step in front of us; i = 2 st + 1: in the middle of a stage
         while (st < stages) {
             if (!(i & 1) && i <= steps) {
@@ -780,17 +828,17 @@ __global__ __launch_bounds__(W_NT, 1) void seq_attention_wide_kernel(const uint1
                 if ((2 * st + 3) * 32 <= all_open) {
                     do {
                         begin_stage();
-                        step(std::false_type(), 2 * st, sc, sn, pc, pn);
+                        step(std::false_type(), std::false_type(), 2 * st, sc, sn, pc, pn);
                         if (some_exceed()) { half = true; break; }
-                        step(std::false_type(), 2 * st + 1, sn, sc, pn, pc);
+                        step(std::false_type(), std::true_type(), 2 * st + 1, sn, sc, pn, pc);
                         st++;
                     } while (!some_exceed() && (2 * st + 3) * 32 <= all_open);
                 } else {
                     do {
                         begin_stage();
-                        step(std::true_type(), 2 * st, sc, sn, pc, pn);
+                        step(std::true_type(), std::false_type(), 2 * st, sc, sn, pc, pn);
                         if (some_exceed()) { half = true; break; }
-                        step(std::true_type(), 2 * st + 1, sn, sc, pn, pc);
+                        step(std::true_type(), std::true_type(), 2 * st + 1, sn, sc, pn, pc);
                         st++;
                     } while (!some_exceed() && 2 * st <= steps && st < stages);
                 }
@@ -806,6 +854,10 @@ __global__ __launch_bounds__(W_NT, 1) void seq_attention_wide_kernel(const uint1
             } else {
                 if (!(i & 1)) begin_stage();
                 if (i <= steps) slow_step(i, sc, pc);
+                if constexpr (PAGED)
+                    if (i & 1)
+#pragma unroll
+                        for (int p = 0; p < G::NI; p++) look_up(st + 4, p);
                 i++;
                 if (!(i & 1)) st++;
             }

@@ -252,20 +252,19 @@ struct AttentionMask {
 int launch_attention(hodu_rocm_ctx *ctx, int dtype, const void *q, const void *k, const void *v, void *out,
                      const AttentionArgs &a, const AttentionMask *mask = nullptr);
 
-// Division of a non-negative 31-bit index by a fixed extent as a multiplication: n / d = n * mul >> sh with
-// sh = 31 + ceil(log2 d) and mul = ceil(2^sh / d).  Exact: mul * d = 2^sh + e with e < d <= 2^(sh - 31), so the excess
-// n * e / (d * 2^sh) stays below 1 / d for n < 2^31.
+// Division of a non-negative 31-bit index by a fixed extent as a multiplication: n / d = n * mul >> (31 + sh) with
+// sh = ceil(log2 d) and mul = ceil(2^(31 + sh) / d), below 2^32.  Exact: mul * d = 2^(31 + sh) + e with e < d <= 2^sh, so the
+// excess n * e / (d * 2^(31 + sh)) stays below 1 / d for n < 2^31.  (The quotient is fixed_quotient, device_types.hpp.)
 struct FixedDiv {
-    unsigned long long mul = 1;
+    unsigned mul = 1u << 31;
     int d = 1, sh = 0;
 };
 inline FixedDiv fixed_div(int d) {
     FixedDiv f;
-    int up = 0;
-    while ((1LL << up) < d) up++;
     f.d = d;
-    f.sh = 31 + up;
-    f.mul = ((1ULL << f.sh) + (unsigned long long)d - 1) / (unsigned long long)d;
+    f.sh = 0;
+    while ((1LL << f.sh) < d) f.sh++;
+    f.mul = (unsigned)(((1ULL << (31 + f.sh)) + (unsigned long long)d - 1) / (unsigned long long)d);
     return f;
 }
 

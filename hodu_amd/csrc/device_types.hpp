@@ -45,6 +45,11 @@ __device__ __forceinline__ void batch_offsets(const DevProduct &g, long batch, l
     }
 }
 
+// n / f.d for 0 <= n < 2^31
+__device__ __forceinline__ int fixed_quotient(int n, const FixedDiv &f) {
+    return (int)((unsigned)(((unsigned long long)((unsigned)n << 1) * f.mul) >> 32) >> f.sh);
+}
+
 // ---- scalar conversions ---------------------------------------------------------------------
 __device__ __forceinline__ float bf16_bits_to_f32(uint16_t h) { return __uint_as_float(((uint32_t)h) << 16); }
 

@@ -6,8 +6,6 @@
 namespace hodu {
 namespace {
 
-__device__ __forceinline__ int fixed_quotient(int n, const FixedDiv &f) { return (int)(((unsigned long long)(unsigned)n * f.mul) >> f.sh); }
-
 // ---- block tables and slot maps -----------------------------------------------------------------------------------
 // held_r = ceil(cached_r / P), need_r = ceil((cached_r + added_r) / P); a request's fresh pages are the next
 // need_r - held_r of the free list, its tokens the next added_r rows: both are running sums over the requests.  The

@@ -158,11 +158,18 @@ inline unsigned slot_u32(const unsigned char (*slots)[kWideBytes], unsigned lane
 inline int readlane(int v, int lane) { return (int)slot_u32(wave_values((unsigned)v), (unsigned)lane & 63u); }
 // v_mov_b32 with a DPP control, all rows and banks enabled: the controls these kernels use
 inline int update_dpp(int old, int src, int ctrl, int row_mask, int bank_mask, bool bound_ctrl) {
-    (void)old; (void)bound_ctrl;
-    if (row_mask != 0xF || bank_mask != 0xF) (void)no_such_instruction("DPP with a row or bank mask");
+    const bool bcast = ctrl == 0x142 || ctrl == 0x143;
+    if ((row_mask != 0xF && !bcast) || bank_mask != 0xF) (void)no_such_instruction("DPP with a row or bank mask");
     const auto slots = wave_values((unsigned)src);
     const unsigned l = lane_id();
+    if (!((row_mask >> (l / 16)) & 1)) return old;  // a row that is not enabled keeps what was there
     unsigned from;
+    if (ctrl >= 0x111 && ctrl <= 0x11F) {            // row_shr: zeros (bound_ctrl) come in from the left
+        const unsigned n = (unsigned)ctrl & 15u;
+        return (l & 15u) >= n ? (int)slot_u32(slots, l - n) : bound_ctrl ? 0 : old;
+    }
+    if (ctrl == 0x142) return l >= 16 ? (int)slot_u32(slots, (l & ~15u) - 1) : old;  // row_bcast:15, each row's last lane to the next row
+    if (ctrl == 0x143) return l >= 32 ? (int)slot_u32(slots, 31) : old;              // row_bcast:31
     if (ctrl >= 0 && ctrl <= 0xFF) from = (l & ~3u) + (((unsigned)ctrl >> (2 * (l & 3u))) & 3u);  // quad_perm
     else if (ctrl == 0x140) from = (l & ~15u) + (15u - (l & 15u));                                 // row_mirror
     else if (ctrl == 0x141) from = (l & ~7u) + (7u - (l & 7u));                                    // row_half_mirror

@@ -196,6 +196,28 @@ def test_every_tile(ctx, tile, dt, cache_dt, d):
         ctx.force_tile(-1)
 
 
+@pytest.mark.parametrize("tile", TILES)
+@pytest.mark.parametrize("cache_dt", ["bf16", "f8e4m3"])
+def test_tables_longer_than_what_a_workgroup_holds_of_them(ctx, tile, cache_dt):
+    """pages of one and of three tokens: the windows of table entries in LDS are filled again and again"""
+    ctx.force_tile(tile)
+    try:
+        S.run_paged(ctx, "bf16", [9, 1], [2500, 1300], 2, 1, 64, 1, cache_dt, seed=240)
+        S.run_paged(ctx, "bf16", [3], [7000], 1, 1, 128, 3, cache_dt, seed=241)
+    finally:
+        ctx.force_tile(-1)
+
+
+def test_many_sequences(ctx):
+    """more than a workgroup looks at in one step of its search"""
+    g = np.random.default_rng(3)
+    for n in (255, 256, 257, 600):
+        lens = (g.integers(0, 3, n) * g.integers(0, 2, n)).tolist()
+        lens[-1] = 2
+        S.run_varlen(ctx, "bf16", lens, lens, 2, 1, 64, True, seed=250, expect="r16")
+        S.run_paged(ctx, "f16", [min(1, x) for x in lens], [x + 3 for x in lens], 2, 2, 64, 4, seed=251)
+
+
 def test_calls_in_a_row_give_the_same_bits(ctx):
     a = S.run_paged(ctx, "bf16", [1, 1, 30], [400, 77, 130], 8, 2, 128, 16, seed=170)
     S.run_paged(ctx, "bf16", [60], [160], 4, 1, 64, 16, seed=171)
