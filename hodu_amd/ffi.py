@@ -264,6 +264,11 @@ def _md_array(md: Sequence[int]):
     return arr, len(md)
 
 
+def _words(md: Sequence[int]):
+    """the same of a sequence that holds plain numbers already (a loop's step calls four times with some twenty each)"""
+    return (ctypes.c_size_t * len(md))(*md), len(md)
+
+
 class DeviceBuffer:
     """A device allocation owned by a Context (what CudaSlice is to the CUDA sibling)."""
 
@@ -297,9 +302,10 @@ class DeviceView:
 
     @classmethod
     def of(cls, tensor) -> "DeviceView":
-        """of a torch tensor: from its first element to the end of its storage"""
-        storage, size = tensor.untyped_storage(), tensor.element_size()
-        return cls(tensor.data_ptr(), storage.nbytes() - tensor.storage_offset() * size)
+        """of a torch tensor: its elements or, where they do not lie side by side, all up to the end of its storage"""
+        if tensor.is_contiguous():
+            return cls(tensor.data_ptr(), tensor.nbytes)
+        return cls(tensor.data_ptr(), tensor.untyped_storage().nbytes() - tensor.storage_offset() * tensor.element_size())
 
 
 class Context:
@@ -525,7 +531,7 @@ class Context:
             for name, buf, n in (("free_pages", free_pages, n_free), ("slots", slots, capacity)):
                 if buf is not None:
                     _within("paged_plan", (name, buf, 4 * n))
-        arr, n = _md_array(md)
+        arr, n = _words(md)
         self._check(self.lib.hodu_rocm_paged_plan(
             self.handle, cached.ptr, added.ptr, None if free_pages is None else free_pages.ptr, table.ptr, lens.ptr, offsets.ptr,
             None if slots is None else slots.ptr, used.ptr, arr, n))
@@ -543,7 +549,7 @@ class Context:
             for name, buf in (("k_scale", k_scale), ("v_scale", v_scale)):
                 if buf is not None:
                     _within("paged_store", (name, buf, 4 * h))
-        arr, n = _md_array(md)
+        arr, n = _words(md)
         self._check(self.lib.hodu_rocm_paged_store(
             self.handle, DTYPE_ID[dt], DTYPE_ID[cache_dt], k.ptr, v.ptr, k_cache.ptr, v_cache.ptr, slots.ptr,
             None if k_scale is None else k_scale.ptr, None if v_scale is None else v_scale.ptr, arr, n))
@@ -557,7 +563,7 @@ class Context:
             _within("attention_varlen", ("q", q, _span3(tq, hq, d, qt, qh, qo) * es), ("k", k, _span3(tk, hk, d, kt, kh, ko) * es),
                     ("v", v, _span3(tk, hk, d, vt, vh, vo) * es), ("out", out, tq * hq * d * es), ("q_offsets", q_offsets, 4 * b + 4),
                     ("k_offsets", k_offsets, 4 * b + 4))
-        arr, n = _md_array(md)
+        arr, n = _words(md)
         sc = np.ascontiguousarray(scale).reshape(1)
         self._check(self.lib.hodu_rocm_attention_varlen(self.handle, DTYPE_ID[dt], q.ptr, k.ptr, v.ptr, out.ptr, q_offsets.ptr,
                                                         k_offsets.ptr, arr, n, sc.ctypes.data, int(bool(causal))))
@@ -578,7 +584,7 @@ class Context:
             for name, buf in (("k_scale", k_scale), ("v_scale", v_scale)):
                 if buf is not None:
                     _within("attention_paged", (name, buf, 4 * hk))
-        arr, n = _md_array(md)
+        arr, n = _words(md)
         sc = np.ascontiguousarray(scale).reshape(1)
         self._check(self.lib.hodu_rocm_attention_paged(
             self.handle, DTYPE_ID[dt], DTYPE_ID[cache_dt], q.ptr, k_cache.ptr, v_cache.ptr, out.ptr, q_offsets.ptr, table.ptr, lens.ptr,

@@ -299,7 +299,7 @@ int hodu_rocm_attention_masked(hodu_rocm_ctx *ctx, int dtype, const void *q, con
  * no token, takes no page, and lens[r] is what was cached (0 if that is negative) -- when a length is negative, when it outgrows `width`
  * pages, when the list holds too few pages for it, or when its tokens pass `capacity`; the list and the capacity are
  * dealt out in order, so once one of them ran out every later request that needs it is refused too.
- * metadata: [batch, page_size, width, n_free, capacity]; at most 16384 requests.  Outputs and inputs must not overlap. */
+ * metadata: [batch, page_size, width, n_free, capacity]; at most 8192 requests.  Outputs and inputs must not overlap. */
 int hodu_rocm_paged_plan(hodu_rocm_ctx *ctx, const int *cached, const int *added, const int *free_pages, int *table, int *lens,
                          int *offsets, int *slots, int *used, const size_t *metadata, size_t metadata_len);
 
