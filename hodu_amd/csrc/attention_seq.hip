@@ -111,6 +111,38 @@ template <int ROWS, bool PAGED> __device__ __forceinline__ bool find_tile(const 
     return false;
 }
 
+// The same for tiles that work for long, of up to 64 sequences: the ones with most keys first and each from its last row, so that
+// the tiles left over at a launch's end are short ones.  A lane owns a sequence, sums the tiles of those before it in that order, and
+// knows whether the tile is its own.
+template <int ROWS, bool PAGED> __device__ __forceinline__ bool find_tile_long_first(const DevSeq &a, int tile, SeqTile &f) {
+    const int lane = threadIdx.x & 63, s = lane < a.batch ? lane : a.batch - 1;
+    const int q = a.q_offsets[s], q_end = a.q_offsets[s + 1];
+    const int k = PAGED ? 0 : a.k_offsets[s], k_end = PAGED ? a.lens[s] : a.k_offsets[s + 1];
+    const int hi = q_end < a.q_tokens ? q_end : a.q_tokens, lo = q > 0 ? q : 0;
+    const int len = lane < a.batch && hi > lo ? hi - lo : 0;
+    const int most = PAGED ? a.width * a.page.d : a.k_tokens, k_hi = k_end < most ? k_end : most, k0 = k > 0 ? k : 0;
+    const int m = k_hi > k0 ? k_hi - k0 : 0;
+    const int tiles = (int)(((long)len * a.group + ROWS - 1) / ROWS);
+    const unsigned order = ((unsigned)(m < (1 << 26) ? m : (1 << 26) - 1) << 6) + (63 - lane);
+    int start = 0;
+    for (int j = 0; j < a.batch; j++) {
+        const unsigned other = (unsigned)__builtin_amdgcn_readlane((int)order, j);
+        const int its = __builtin_amdgcn_readlane(tiles, j);
+        start += other > order ? its : 0;
+    }
+    const unsigned long long mine = __builtin_amdgcn_ballot_w64(tile >= start && tile - start < tiles);
+    if (!mine) return false;
+    const int at = __builtin_ctzll(mine);
+    f.b = at;
+    f.row0 = (__builtin_amdgcn_readlane(tiles, at) - 1 - (tile - __builtin_amdgcn_readlane(start, at))) * ROWS;
+    f.q0 = __builtin_amdgcn_readlane(lo, at);
+    f.n = __builtin_amdgcn_readlane(len, at);
+    f.k0 = __builtin_amdgcn_readlane(k0, at);
+    f.m = __builtin_amdgcn_readlane(m, at);
+    // (offsets that do not ascend can make the sums above wrap; a tile outside its sequence is no tile)
+    return f.row0 >= 0 && f.row0 < (long)f.n * a.group;
+}
+
 template <int CK> __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     typedef float f32x2 __attribute__((ext_vector_type(2)));
     if constexpr (CK == mfma::CK_BF16) {
@@ -449,7 +481,7 @@ __global__ __launch_bounds__(R16_NT) void seq_attention_r16_kernel(const uint16_
 // Row tiles per wavefront: 3 at head dim 128 (O, q, two steps' scores and P are 84 registers a tile; with 4 the allocator runs out),
 // 4 at 64.
 template <int D> constexpr int W_TILES = D == 128 ? 3 : 4;
-constexpr int W_NT = 256, W_BK = 64, W_RING = 4, W_WINDOW = 2048;  // (the ring: stages of K and of V)
+constexpr int W_NT = 256, W_BK = 64, W_RING = 4, W_WINDOW = 2048, W_MIN_STAGES = 8;  // (the ring: stages of K and of V)
 template <int D, bool F8, bool PAGED> struct WGeom : SeqGeom<D, F8> {
     typedef SeqGeom<D, F8> S;
     static constexpr int NI = 2 * S::DMAS / 4;               // LDS-DMA instructions per stage of K (of V) and wavefront
@@ -459,7 +491,8 @@ template <int D, bool F8, bool PAGED> struct WGeom : SeqGeom<D, F8> {
 
 template <int CK, int D, bool PAGED, bool F8, int RT>
 __global__ __launch_bounds__(W_NT, 1) void seq_attention_wide_kernel(const uint16_t *__restrict__ Q, const char *__restrict__ K,
-                                                                     const char *__restrict__ V, uint16_t *__restrict__ O, DevSeq a) {
+                                                                     const char *__restrict__ V, uint16_t *__restrict__ O, DevSeq a,
+                                                                     float *ws, unsigned ws_bytes, int *arrival) {
     typedef WGeom<D, F8, PAGED> G;
     typedef Compute<CK> Cmp;
     typedef typename Cmp::acc_t acc_t;
@@ -470,7 +503,8 @@ __global__ __launch_bounds__(W_NT, 1) void seq_attention_wide_kernel(const uint1
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 15, g = lane >> 4;
     const int kvh = blockIdx.x % a.kv_heads;
     SeqTile f;
-    if (!find_tile<BM, PAGED>(a, blockIdx.x / a.kv_heads, f)) return;
+    const int tile = blockIdx.x / a.kv_heads;
+    if (!(a.batch <= 64 ? find_tile_long_first<BM, PAGED>(a, tile, f) : find_tile<BM, PAGED>(a, tile, f))) return;
     const int b = f.b, row0 = f.row0, q0 = f.q0, n = f.n, k0 = f.k0, m = f.m, rows = n * a.group;
     // the lane's rows, one per tile; rows past the sequence's last repeat it and are not stored
     int open[RT];
@@ -488,23 +522,40 @@ __global__ __launch_bounds__(W_NT, 1) void seq_attention_wide_kernel(const uint1
     const float c = a.scale_log2e * (F8 ? a.k_scale[kvh] : 1.f);
     auto last_row = [&](int i) { return i < rows ? i : rows - 1; };
     const int keys_any = a.causal ? quot(last_row(row0 + BM - 1), a.by_group) + m - n + 1 : m;  // keys the tile needs
-    const int keys = keys_any > 0 ? keys_any : 0;
-    const int wave_keys = a.causal ? quot(last_row(wrow0 + 16 * RT - 1), a.by_group) + m - n + 1 : m;  // ... the wavefront needs
-    const int all_open = a.causal ? quot(last_row(wrow0), a.by_group) + m - n + 1 : m;  // keys below this are open to all its rows
-    const int stages = (keys + W_BK - 1) / W_BK;
+    int keys = keys_any > 0 ? keys_any : 0;
+    int wave_keys = a.causal ? quot(last_row(wrow0 + 16 * RT - 1), a.by_group) + m - n + 1 : m;  // ... the wavefront needs
+    int all_open = a.causal ? quot(last_row(wrow0), a.by_group) + m - n + 1 : m;  // keys below this are open to all its rows
+    int stages = (keys + W_BK - 1) / W_BK;
+    // few tiles over a long cache: this workgroup's range of the keys, and everything from here on counts from its first one
+    int from = 0, splits = 1;
+    if constexpr (PAGED) {
+        const int worth = stages / W_MIN_STAGES, split = blockIdx.y;
+        splits = worth < 1 ? 1 : worth < (int)gridDim.y ? worth : (int)gridDim.y;
+        if (split >= splits) return;
+        if (splits > 1) {
+            const int s0 = stages * split / splits, s1 = stages * (split + 1) / splits;
+            from = s0 * W_BK;
+            stages = s1 - s0;
+            keys = (keys < s1 * W_BK ? keys : s1 * W_BK) - from;
+            wave_keys = wave_keys - from < keys ? wave_keys - from : keys;
+            all_open = all_open - from < keys ? all_open - from : keys;
+#pragma unroll
+            for (int x = 0; x < RT; x++) open[x] -= from;
+        }
+    }
     const int steps = wave_keys > 0 && wrow0 < rows ? (wave_keys + 31) / 32 : 0;  // of 32 keys, that the wavefront needs
 
     // ---- memory -> LDS: instruction i of a block fills 1 KB, KPI keys; a wavefront issues NI of them for K and for V ----
     const char *kbase = K + kvh * a.kc.head, *vbase = V + kvh * a.vc.head;
     int *window = reinterpret_cast<int *>(smem + G::TABLE_AT);
     int window0 = 0;  // first table column in the window
-    [[maybe_unused]] auto fill_window = [&](int from) __attribute__((always_inline)) {
-        const int cols = quot(keys - 1, a.page) + 1;
-        for (int i = tid; i < W_WINDOW && from + i < cols; i += W_NT) {
-            const int pg = a.table[(long)b * a.width + from + i];
+    [[maybe_unused]] auto fill_window = [&](int col0) __attribute__((always_inline)) {
+        const int cols = quot(from + keys - 1, a.page) + 1;
+        for (int i = tid; i < W_WINDOW && col0 + i < cols; i += W_NT) {
+            const int pg = a.table[(long)b * a.width + col0 + i];
             window[i] = pg < 0 ? 0 : pg < a.n_pages ? pg : a.n_pages - 1;
         }
-        window0 = from;
+        window0 = col0;
     };
     // a lane's source within a stage of packed keys (the token stride is below 2^25 bytes: the host sees to it)
     unsigned in_stage[2][G::NI];
@@ -519,7 +570,7 @@ __global__ __launch_bounds__(W_NT, 1) void seq_attention_wide_kernel(const uint1
     [[maybe_unused]] int k_page[G::NI], k_in[G::NI], v_page[G::NI], v_in[G::NI];
     auto look_up = [&](int stage, int p) __attribute__((always_inline)) {
         int key = stage * W_BK + (wave * G::NI + p) * G::KPI + lane / G::CPR;
-        key = key < keys ? key : keys - 1;  // behind the last key: that one again, masked below
+        key = from + (key < keys ? key : keys - 1);  // behind the last key: that one again, masked below
         const int col = quot(key, a.page);
         k_page[p] = window[col - window0];
         k_in[p] = key - col * a.page.d;
@@ -535,9 +586,9 @@ __global__ __launch_bounds__(W_NT, 1) void seq_attention_wide_kernel(const uint1
         // (a stage is two blocks of 32 keys, the ring eight)
         const unsigned to = lds0 + (is_v ? G::V_AT : 0) + (stage & (W_RING - 1)) * 2 * (is_v ? G::BLOCK_V : G::BLOCK_K) + wave * G::NI * padded;
         if (!PAGED && (stage + 1) * W_BK <= keys) {
-            const char *from = base + (long)(k0 + stage * W_BK) * side.token;
+            const char *keys0 = base + (long)(k0 + stage * W_BK) * side.token;
 #pragma unroll
-            for (int p = 0; p < G::NI; p++) mfma::dma16_sbase(from, in_stage[is_v][p], __builtin_amdgcn_readfirstlane(to + p * padded));
+            for (int p = 0; p < G::NI; p++) mfma::dma16_sbase(keys0, in_stage[is_v][p], __builtin_amdgcn_readfirstlane(to + p * padded));
             return;
         }
 #pragma unroll
@@ -764,7 +815,7 @@ __global__ __launch_bounds__(W_NT, 1) void seq_attention_wide_kernel(const uint1
 
     if (stages > 0) {
         if constexpr (PAGED) {
-            fill_window(0);
+            fill_window(quot(from, a.page));
             __syncthreads();
         }
         // step 0 multiplies a P of zeros by what lies where V of the step before it would: zeros too
@@ -801,10 +852,10 @@ __global__ __launch_bounds__(W_NT, 1) void seq_attention_wide_kernel(const uint1
             if constexpr (PAGED) {
                 pass_on();
                 // the table columns of the keys that are looked up in this stage, K of stage st + 4
-                const int hi = (st + 5) * W_BK - 1 < keys ? (st + 5) * W_BK - 1 : keys - 1;
+                const int hi = from + ((st + 5) * W_BK - 1 < keys ? (st + 5) * W_BK - 1 : keys - 1);
                 if (st + 4 < stages && quot(hi, a.page) - window0 >= W_WINDOW) {
                     __syncthreads();  // (everybody has looked up what the window held)
-                    fill_window(quot((st + 4) * W_BK, a.page));
+                    fill_window(quot(from + (st + 4) * W_BK, a.page));
                     __syncthreads();
                 }
             }
@@ -866,6 +917,54 @@ __global__ __launch_bounds__(W_NT, 1) void seq_attention_wide_kernel(const uint1
         if (steps == 2 * stages) times_v(steps - 1, pc);  // P V of the last step
     }
 
+    if constexpr (PAGED) {
+        if (splits > 1) {
+            // A range leaves (reference, sum) and O of its rows, 16 bytes of each lane side by side; the tile's last one to arrive adds
+            // them in the order of the ranges.
+            constexpr unsigned WAVE = RT * (DT + 1) * 1024, SLICE = 4 * WAVE;
+            const __amdgpu_buffer_rsrc_t buf = agent_buffer(ws, ws_bytes);
+            const unsigned tile_at = blockIdx.x * gridDim.y * SLICE + wave * WAVE + lane * 16, mine = tile_at + blockIdx.y * SLICE;
+            if (wrow0 < rows) {
+#pragma unroll
+                for (int x = 0; x < RT; x++) {
+                    store16_agent(buf, mine + x * (DT + 1) * 1024, f32x4_t{e_ref[x], o[x][DT][0], 0.f, 0.f});
+#pragma unroll
+                    for (int j = 0; j < DT; j++)
+                        store16_agent(buf, mine + (x * (DT + 1) + 1 + j) * 1024, f32x4_t{o[x][j][0], o[x][j][1], o[x][j][2], o[x][j][3]});
+                }
+            }
+            if (!arrive_and_check_last(arrival + blockIdx.x, splits, reinterpret_cast<int *>(smem), tid)) return;
+            if (wrow0 < rows) {
+#pragma unroll
+                for (int x = 0; x < RT; x++) {
+                    const unsigned row_at = tile_at + x * (DT + 1) * 1024;
+                    float e_all = -1e30f, l = 0.f;
+                    for (int i = 0; i < splits; i++) e_all = __builtin_fmaxf(e_all, load16_agent<f32x4_t>(buf, row_at + i * SLICE).x);
+                    f32x4_t y[DT];
+#pragma unroll
+                    for (int j = 0; j < DT; j++) y[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+                    for (int i = 0; i < splits; i++) {
+                        const f32x4_t h = load16_agent<f32x4_t>(buf, row_at + i * SLICE);
+                        const float w = __builtin_amdgcn_exp2f(h.x - e_all);
+                        l += h.y * w;
+#pragma unroll
+                        for (int j = 0; j < DT; j++) {
+                            const f32x4_t part = load16_agent<f32x4_t>(buf, row_at + i * SLICE + (1 + j) * 1024);
+#pragma unroll
+                            for (int e = 0; e < 4; e++) y[j][e] += part[e] * w;
+                        }
+                    }
+                    o[x][DT][0] = l;
+#pragma unroll
+                    for (int j = 0; j < DT; j++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) o[x][j][e] = y[j][e];
+                }
+            }
+            arrival_reset(arrival + blockIdx.x, tid);
+        }
+    }
+
     // ---- O / l, one rounding: lane (r, g) holds row r of each tile, head-dim columns 16 j + 4 g + e ----
 #pragma unroll
     for (int x = 0; x < RT; x++) {
@@ -916,13 +1015,37 @@ int launch_seq_attention(hodu_rocm_ctx *ctx, int dtype, int cache_dtype, const v
     const char *kp = (const char *)k + g.kc.off * es, *vp = (const char *)v + g.vc.off * es;
     // rows of a sequence and key / value head, on average
     const long sequences = g.q_tokens < g.batch ? g.q_tokens : g.batch, avg_rows = g.q_tokens * a.group / sequences;
-    auto launch = [&](auto kernel, int rows, int nt, int lds, const char *name) -> int {
+    const long cus = ctx->props.multiProcessorCount;
+    // A launch of wide tiles, with the keys of a tile in `splits` ranges
+    auto launch = [&](auto kernel, int rows, int d, int splits, int lds, const char *name) -> int {
         const long blocks = (sequences + g.q_tokens * a.group / rows) * g.kv_heads;
         if (blocks > 0x7FFFFFFFL) return HODU_ROCM_UNSUPPORTED;
+        if (blocks > kArrivalSlots) splits = 1;
+        const size_t ws_bytes = splits > 1 ? (size_t)blocks * splits * rows * (d + 16) * 4 : 0;
+        if (splits > 1) {
+            if (int rc = ensure_workspace(ctx, ws_bytes)) return rc;
+            if (int rc = ensure_arrival(ctx)) return rc;
+        }
         if (int rc = ensure_dynamic_lds(ctx, reinterpret_cast<const void *>(kernel), lds)) return rc;
         ctx->last_kernel = name;
-        hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(nt), lds, ctx->stream, qp, kp, vp, (uint16_t *)out, a);
+        hipLaunchKernelGGL(kernel, dim3((unsigned)blocks, (unsigned)splits), dim3(W_NT), lds, ctx->stream, qp, kp, vp, (uint16_t *)out, a,
+                           (float *)ctx->workspace.ptr, (unsigned)ws_bytes, ctx->arrival);
         return HODU_ROCM_OK;
+    };
+    // What a launch of wide tiles takes, in ns: a compute unit works on one at a time, so whole rounds of (what a workgroup costs however
+    // short it is, what meeting adds, its stages).  Few tiles over a long cache fill the rounds by cutting the keys; the workspace
+    // bounds that at four workgroups per compute unit.
+    const long keys = g.paged ? (long)a.width * a.page.d : g.k_tokens / sequences, max_stages = (keys + W_BK - 1) / W_BK;
+    struct Wide { int rows, splits; long ns; };
+    auto wide = [&](int rows, long stage_ns) {
+        const long tiles = sequences * ((avg_rows + rows - 1) / rows) * g.kv_heads;
+        Wide best{rows, 1, 0};
+        for (int s = 1; s <= 16; s++) {
+            if (s > 1 && (!g.paged || s * W_MIN_STAGES > max_stages || s * tiles > 4 * cus)) break;
+            const long ns = (tiles * s + cus - 1) / cus * (11000 + (s > 1 ? 5000 + s * 500 : 0) + max_stages * stage_ns / s);
+            if (s == 1 || ns < best.ns) best.splits = s, best.ns = ns;
+        }
+        return best;
     };
     auto by_form = [&](auto ck, auto d, auto paged, auto f8_) -> int {
         constexpr int CK = decltype(ck)::value, D = decltype(d)::value;
@@ -930,18 +1053,21 @@ int launch_seq_attention(hodu_rocm_ctx *ctx, int dtype, int cache_dtype, const v
         // packed keys of the wide kernels: a stage's keys by a 32-bit offset
         const bool near = PAGED || (a.kc.token < (1L << 25) && a.vc.token < (1L << 25));
         const int pin = ctx->force_tile;  // testing hook: 50 tiles of 16 rows, 51 of 128, 52 of 192 or 256
-        if (near && (pin == 52 || (pin < 50 && avg_rows >= 192)))
-            return launch(seq_attention_wide_kernel<CK, D, PAGED, F8, W_TILES<D>>, 64 * W_TILES<D>, W_NT, WGeom<D, F8, PAGED>::LDS,
+        constexpr int BIG = 64 * W_TILES<D>;
+        const Wide small = wide(128, D == 128 ? 1400 : 950), big = wide(BIG, D == 128 ? 1750 : 1450);
+        const bool wide_rows = avg_rows >= (PAGED ? 17 : 48);
+        if (near && (pin == 52 || (pin < 50 && wide_rows && big.ns < small.ns)))
+            return launch(seq_attention_wide_kernel<CK, D, PAGED, F8, W_TILES<D>>, BIG, D, big.splits, WGeom<D, F8, PAGED>::LDS,
                           !PAGED ? "attention_varlen_wide" : F8 ? "attention_paged_wide_f8" : "attention_paged_wide");
-        if (near && (pin == 51 || (pin < 50 && avg_rows >= 48)))
-            return launch(seq_attention_wide_kernel<CK, D, PAGED, F8, 2>, 128, W_NT, WGeom<D, F8, PAGED>::LDS,
+        if (near && (pin == 51 || (pin < 50 && wide_rows)))
+            return launch(seq_attention_wide_kernel<CK, D, PAGED, F8, 2>, 128, D, small.splits, WGeom<D, F8, PAGED>::LDS,
                           !PAGED ? "attention_varlen_wide128" : F8 ? "attention_paged_wide128_f8" : "attention_paged_wide128");
         // Few tiles over long contexts: the keys are cut across workgroups, to about eight per compute unit (they differ in
         // length, and the last ones of a launch should be short).  How many of them a tile uses goes by its keys, on the device.
         typedef R16Geom<D, F8> G;
         const long tiles = (sequences + g.q_tokens * a.group / R16) * g.kv_heads;
         const long most_keys = PAGED ? (long)a.width * a.page.d : g.k_tokens;
-        long splits = 8L * ctx->props.multiProcessorCount / tiles;
+        long splits = 8 * cus / tiles;
         const long worth = (most_keys / R16_BK + R16_MIN_BLOCKS) / R16_MIN_BLOCKS;
         splits = splits > worth ? worth : splits;
         splits = splits > 64 ? 64 : splits;

@@ -208,6 +208,20 @@ def test_tables_longer_than_what_a_workgroup_holds_of_them(ctx, tile, cache_dt):
         ctx.force_tile(-1)
 
 
+@pytest.mark.parametrize("tile", TILES)
+@pytest.mark.parametrize("dt,cache_dt,d", [("bf16", "bf16", 128), ("f16", "f16", 64), ("bf16", "f8e4m3", 64), ("f16", "f8e4m3", 128)])
+def test_keys_cut_across_workgroups(ctx, tile, dt, cache_dt, d):
+    """few tiles over long caches: a sequence that is cut often, one that is not, one whose first rows attend nothing of the last range"""
+    ctx.force_tile(tile)
+    try:
+        for _ in range(2):  # (the second finds the counters as the first left them)
+            S.run_paged(ctx, dt, [20, 0, 7, 1], [2900, 600, 1100, 40], 4, 1, d, 16, cache_dt, seed=260)
+        S.run_paged(ctx, dt, [520], [1300], 1, 1, d, 64, cache_dt, seed=261, garbage=0x7F if cache_dt == "f8e4m3" else 0x7F80)
+        S.run_paged(ctx, dt, [30, 3], [1100, 1500], 2, 2, d, 3, cache_dt, seed=262)
+    finally:
+        ctx.force_tile(-1)
+
+
 def test_many_sequences(ctx):
     """more than a workgroup looks at in one step of its search"""
     g = np.random.default_rng(3)
