@@ -179,7 +179,7 @@ template <int CK> __device__ __forceinline__ u32x4_t widen8(const u32x2_t &v) {
 //
 // A tile's workgroups meet through the workspace (agent_scope.hpp): each leaves its rows' (reference, sum, O), the last one
 // to arrive adds them in range order, so the result does not depend on who was last.
-constexpr int R16 = 16, R16_NT = 256, R16_BK = 32, R16_WINDOW = 256;
+constexpr int R16 = 16, R16_WAVES = 4, R16_NT = 64 * R16_WAVES, R16_BK = 32, R16_WINDOW = 256;
 constexpr int R16_MIN_BLOCKS = 4;  // blocks of a workgroup below which keys are not cut further: one per wavefront
 template <int D, bool F8> struct SeqGeom {
     static_assert(D == 64 || D == 128, "head dim");
@@ -215,9 +215,9 @@ template <int D, bool F8> struct R16Geom : SeqGeom<D, F8> {
     static constexpr int RING = S::DMAS == 8 ? 2 : 4;        // blocks of K and of V in a wavefront's ring
     static constexpr int BLOCK = S::BLOCK_K + S::BLOCK_V, WAVE = RING * BLOCK;
     static constexpr int LINE = D + 4;                       // floats of a row's (reference, sum, -, -, O)
-    static constexpr int MERGE = 4 * R16 * LINE * 4;
-    static constexpr int WINDOW_AT = 4 * WAVE > MERGE ? 4 * WAVE : MERGE;
-    static constexpr int LDS = WINDOW_AT + 4 * R16_WINDOW * 4 + 16;
+    static constexpr int MERGE = R16_WAVES * R16 * LINE * 4;
+    static constexpr int WINDOW_AT = R16_WAVES * WAVE > MERGE ? R16_WAVES * WAVE : MERGE;
+    static constexpr int LDS = WINDOW_AT + R16_WAVES * R16_WINDOW * 4 + 16;
 };
 // 1.0 in every element: the row sums are one more tile of the second product, over the P that it multiplies (which is rounded,
 // so that the weights sum to one), and cost no vector instruction and no exchange between a row's lanes
@@ -238,7 +238,8 @@ __global__ __launch_bounds__(R16_NT) void seq_attention_r16_kernel(const uint16_
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 15, g = lane >> 4;
     const int kvh = blockIdx.x % a.kv_heads;
     SeqTile f;
-    if (!find_tile<R16, PAGED>(a, blockIdx.x / a.kv_heads, f)) return;
+    const int tile = blockIdx.x / a.kv_heads;
+    if (!(a.batch <= 64 ? find_tile_long_first<R16, PAGED>(a, tile, f) : find_tile<R16, PAGED>(a, tile, f))) return;
     const int row0 = f.row0, q0 = f.q0, n = f.n, m = f.m, rows = n * a.group;
 
     // the lane's row; rows past the sequence's last repeat it and are not stored
@@ -254,7 +255,7 @@ __global__ __launch_bounds__(R16_NT) void seq_attention_r16_kernel(const uint16_
     const int splits = worth < 1 ? 1 : worth < (int)gridDim.y ? worth : (int)gridDim.y;
     const int split = blockIdx.y;
     if (split >= splits) return;
-    const int blk0 = (int)((long)blocks * (split * 4 + wave) / (splits * 4)), blk1 = (int)((long)blocks * (split * 4 + wave + 1) / (splits * 4));
+    const int blk0 = (int)((long)blocks * (split * R16_WAVES + wave) / (splits * R16_WAVES)), blk1 = (int)((long)blocks * (split * R16_WAVES + wave + 1) / (splits * R16_WAVES));
 
     u32x4_t qf[G::KS];
 #pragma unroll
@@ -410,15 +411,15 @@ __global__ __launch_bounds__(R16_NT) void seq_attention_r16_kernel(const uint16_
         for (int j = 0; j < G::DT; j++) *reinterpret_cast<f32x4_t *>(mine + 4 + 16 * j + 4 * g) = f32x4_t{o[j][0], o[j][1], o[j][2], o[j][3]};
     }
     __syncthreads();
-    const int row = tid >> 4, part = tid & 15;  // 16 threads a row, D / 16 elements each
-    constexpr int PER = D / 16;
+    constexpr int PARTS = R16_NT / R16, PER = D / PARTS;  // threads of a row, elements of each
+    const int row = tid / PARTS, part = tid % PARTS;
     float e_all = -1e30f, l = 0.f, x[PER];
 #pragma unroll
-    for (int i = 0; i < 4; i++) e_all = __builtin_fmaxf(e_all, mg[(i * R16 + row) * G::LINE]);
+    for (int i = 0; i < R16_WAVES; i++) e_all = __builtin_fmaxf(e_all, mg[(i * R16 + row) * G::LINE]);
 #pragma unroll
     for (int e = 0; e < PER; e++) x[e] = 0.f;
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
+    for (int i = 0; i < R16_WAVES; i++) {
         const float *line = mg + (i * R16 + row) * G::LINE;
         const float w = __builtin_amdgcn_exp2f(line[0] - e_all);
         l += line[1] * w;
@@ -431,23 +432,37 @@ __global__ __launch_bounds__(R16_NT) void seq_attention_r16_kernel(const uint16_
         if (part == 0) store16_agent(buf, mine, f32x4_t{e_all, l, 0.f, 0.f});
 #pragma unroll
         for (int e = 0; e < PER; e += 4) store16_agent(buf, mine + (4 + part * PER + e) * 4, f32x4_t{x[e], x[e + 1], x[e + 2], x[e + 3]});
-        int *flag = reinterpret_cast<int *>(smem + G::WINDOW_AT + 4 * R16_WINDOW * 4);
+        int *flag = reinterpret_cast<int *>(smem + G::WINDOW_AT + R16_WAVES * R16_WINDOW * 4);
         if (!arrive_and_check_last(arrival + blockIdx.x, splits, flag, tid)) return;
+        // (eight ranges' loads in flight at once: each is a trip to memory)
         e_all = -1e30f;
-        for (int i = 0; i < splits; i++) e_all = __builtin_fmaxf(e_all, load16_agent<f32x4_t>(buf, tile_at + (i * R16 + row) * G::LINE * 4).x);
         l = 0.f;
 #pragma unroll
         for (int e = 0; e < PER; e++) x[e] = 0.f;
-        for (int i = 0; i < splits; i++) {
-            const unsigned at = tile_at + (i * R16 + row) * G::LINE * 4;
-            const f32x4_t h = load16_agent<f32x4_t>(buf, at);
-            const float w = __builtin_amdgcn_exp2f(h.x - e_all);
-            l += h.y * w;
+        for (int i0 = 0; i0 < splits; i0 += 8) {
+            f32x4_t h[8], y[8][PER / 4];
+            float top = e_all;
 #pragma unroll
-            for (int e = 0; e < PER; e += 4) {
-                const f32x4_t y = load16_agent<f32x4_t>(buf, at + (4 + part * PER + e) * 4);
+            for (int u = 0; u < 8; u++) {
+                const unsigned at = tile_at + ((i0 + u < splits ? i0 + u : splits - 1) * R16 + row) * G::LINE * 4;
+                h[u] = load16_agent<f32x4_t>(buf, at);
 #pragma unroll
-                for (int q = 0; q < 4; q++) x[e + q] += y[q] * w;
+                for (int e = 0; e < PER / 4; e++) y[u][e] = load16_agent<f32x4_t>(buf, at + (4 + part * PER + 4 * e) * 4);
+            }
+#pragma unroll
+            for (int u = 0; u < 8; u++) top = __builtin_fmaxf(top, h[u].x);
+            const float f = __builtin_amdgcn_exp2f(e_all - top);
+            e_all = top;
+            l *= f;
+#pragma unroll
+            for (int e = 0; e < PER; e++) x[e] *= f;
+#pragma unroll
+            for (int u = 0; u < 8; u++) {
+                if (i0 + u >= splits) break;
+                const float w = __builtin_amdgcn_exp2f(h[u].x - e_all);
+                l += h[u].y * w;
+#pragma unroll
+                for (int e = 0; e < PER; e++) x[e] += y[u][e / 4][e % 4] * w;
             }
         }
         arrival_reset(arrival + blockIdx.x, tid);
@@ -459,7 +474,9 @@ __global__ __launch_bounds__(R16_NT) void seq_attention_r16_kernel(const uint16_
 #pragma unroll
     for (int e = 0; e < PER; e += 2) out[e / 2] = pack2<CK>(x[e] * inv, x[e + 1] * inv);
     uint16_t *dst = O + ((long)(q0 + wtok) * a.heads + whead) * D + part * PER;
-    if constexpr (PER == 8) *reinterpret_cast<u32x4_t *>(dst) = u32x4_t{out[0], out[1], out[2], out[3]};
+    if constexpr (PER >= 8)
+#pragma unroll
+        for (int e = 0; e < PER / 2; e += 4) *reinterpret_cast<u32x4_t *>(dst + 2 * e) = u32x4_t{out[e], out[e + 1], out[e + 2], out[e + 3]};
     else *reinterpret_cast<u32x2_t *>(dst) = u32x2_t{out[0], out[1]};
 }
 
@@ -596,7 +613,8 @@ __global__ __launch_bounds__(W_NT, 1) void seq_attention_wide_kernel(const uint1
             const int kk = (wave * G::NI + p) * G::KPI + lane / G::CPR;
             long off;
             if constexpr (PAGED) {
-                off = (is_v ? v_page[p] : k_page[p]) * side.page + (is_v ? v_in[p] : k_in[p]) * side.token;
+                // (32-bit strides, and a page's tokens are within 2^32 bytes: the host sees to it)
+                off = (unsigned long)(unsigned)(is_v ? v_page[p] : k_page[p]) * (unsigned)side.page + (unsigned)(is_v ? v_in[p] : k_in[p]) * (unsigned)side.token;
             } else {
                 int key = stage * W_BK + kk;
                 key = key < keys ? key : keys - 1;  // behind the last key: that one again, masked below
@@ -939,19 +957,38 @@ __global__ __launch_bounds__(W_NT, 1) void seq_attention_wide_kernel(const uint1
                 for (int x = 0; x < RT; x++) {
                     const unsigned row_at = tile_at + x * (DT + 1) * 1024;
                     float e_all = -1e30f, l = 0.f;
-                    for (int i = 0; i < splits; i++) e_all = __builtin_fmaxf(e_all, load16_agent<f32x4_t>(buf, row_at + i * SLICE).x);
                     f32x4_t y[DT];
 #pragma unroll
                     for (int j = 0; j < DT; j++) y[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-                    for (int i = 0; i < splits; i++) {
-                        const f32x4_t h = load16_agent<f32x4_t>(buf, row_at + i * SLICE);
-                        const float w = __builtin_amdgcn_exp2f(h.x - e_all);
-                        l += h.y * w;
+                    // (four ranges' loads in flight at once)
+                    for (int i0 = 0; i0 < splits; i0 += 4) {
+                        f32x4_t h[4], part[4][DT];
+                        float most = e_all;
 #pragma unroll
-                        for (int j = 0; j < DT; j++) {
-                            const f32x4_t part = load16_agent<f32x4_t>(buf, row_at + i * SLICE + (1 + j) * 1024);
+                        for (int u = 0; u < 4; u++) {
+                            const unsigned at = row_at + (i0 + u < splits ? i0 + u : splits - 1) * SLICE;
+                            h[u] = load16_agent<f32x4_t>(buf, at);
 #pragma unroll
-                            for (int e = 0; e < 4; e++) y[j][e] += part[e] * w;
+                            for (int j = 0; j < DT; j++) part[u][j] = load16_agent<f32x4_t>(buf, at + (1 + j) * 1024);
+                        }
+#pragma unroll
+                        for (int u = 0; u < 4; u++) most = __builtin_fmaxf(most, h[u].x);
+                        const float f = __builtin_amdgcn_exp2f(e_all - most);
+                        e_all = most;
+                        l *= f;
+#pragma unroll
+                        for (int j = 0; j < DT; j++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++) y[j][e] *= f;
+#pragma unroll
+                        for (int u = 0; u < 4; u++) {
+                            if (i0 + u >= splits) break;
+                            const float w = __builtin_amdgcn_exp2f(h[u].x - e_all);
+                            l += h[u].y * w;
+#pragma unroll
+                            for (int j = 0; j < DT; j++)
+#pragma unroll
+                                for (int e = 0; e < 4; e++) y[j][e] += part[u][j][e] * w;
                         }
                     }
                     o[x][DT][0] = l;
@@ -1050,24 +1087,27 @@ int launch_seq_attention(hodu_rocm_ctx *ctx, int dtype, int cache_dtype, const v
     auto by_form = [&](auto ck, auto d, auto paged, auto f8_) -> int {
         constexpr int CK = decltype(ck)::value, D = decltype(d)::value;
         constexpr bool PAGED = decltype(paged)::value, F8 = decltype(f8_)::value;
-        // packed keys of the wide kernels: a stage's keys by a 32-bit offset
-        const bool near = PAGED || (a.kc.token < (1L << 25) && a.vc.token < (1L << 25));
+        // the wide kernels address the keys of a stage, or those of a page, by 32-bit offsets (64-bit ones cost them 7 %, the
+        // kernel for 16 rows nothing: it takes what lies further apart)
+        const bool near = PAGED ? a.kc.page < (1L << 32) && a.vc.page < (1L << 32) && a.kc.token < (1L << 32) / a.page.d && a.vc.token < (1L << 32) / a.page.d
+                                : a.kc.token < (1L << 25) && a.vc.token < (1L << 25);
         const int pin = ctx->force_tile;  // testing hook: 50 tiles of 16 rows, 51 of 128, 52 of 192 or 256
         constexpr int BIG = 64 * W_TILES<D>;
         const Wide small = wide(128, D == 128 ? 1400 : 950), big = wide(BIG, D == 128 ? 1750 : 1450);
-        const bool wide_rows = avg_rows >= (PAGED ? 17 : 48);
+        const bool wide_rows = avg_rows > 2 * R16;
         if (near && (pin == 52 || (pin < 50 && wide_rows && big.ns < small.ns)))
             return launch(seq_attention_wide_kernel<CK, D, PAGED, F8, W_TILES<D>>, BIG, D, big.splits, WGeom<D, F8, PAGED>::LDS,
                           !PAGED ? "attention_varlen_wide" : F8 ? "attention_paged_wide_f8" : "attention_paged_wide");
         if (near && (pin == 51 || (pin < 50 && wide_rows)))
             return launch(seq_attention_wide_kernel<CK, D, PAGED, F8, 2>, 128, D, small.splits, WGeom<D, F8, PAGED>::LDS,
                           !PAGED ? "attention_varlen_wide128" : F8 ? "attention_paged_wide128_f8" : "attention_paged_wide128");
-        // Few tiles over long contexts: the keys are cut across workgroups, to about eight per compute unit (they differ in
-        // length, and the last ones of a launch should be short).  How many of them a tile uses goes by its keys, on the device.
+        // Few tiles over long contexts: the keys are cut across workgroups, to about four per compute unit (64 sequences of up to 8192
+        // tokens: 254 us with two and with four, 270 with six, 286 with eight: a workgroup costs some 5 us however short it is).
+        // How many of them a tile uses goes by its keys, on the device.
         typedef R16Geom<D, F8> G;
         const long tiles = (sequences + g.q_tokens * a.group / R16) * g.kv_heads;
         const long most_keys = PAGED ? (long)a.width * a.page.d : g.k_tokens;
-        long splits = 8 * cus / tiles;
+        long splits = 4 * cus / tiles;
         const long worth = (most_keys / R16_BK + R16_MIN_BLOCKS) / R16_MIN_BLOCKS;
         splits = splits > worth ? worth : splits;
         splits = splits > 64 ? 64 : splits;
