@@ -180,7 +180,7 @@ template <int CK> __device__ __forceinline__ u32x4_t widen8(const u32x2_t &v) {
 // A tile's workgroups meet through the workspace (agent_scope.hpp): each leaves its rows' (reference, sum, O), the last one
 // to arrive adds them in range order, so the result does not depend on who was last.
 constexpr int R16 = 16, R16_WAVES = 4, R16_NT = 64 * R16_WAVES, R16_BK = 32, R16_WINDOW = 256;
-constexpr int R16_MIN_BLOCKS = 4;  // blocks of a workgroup below which keys are not cut further: one per wavefront
+constexpr int R16_MIN_BLOCKS = 8;  // blocks of a workgroup below which keys are not cut further: two per wavefront (1999 keys: 12.0 us; with one or four 13.3, 12.2)
 template <int D, bool F8> struct SeqGeom {
     static_assert(D == 64 || D == 128, "head dim");
     static constexpr int ES = F8 ? 1 : 2, ROW = D * ES, CPR = ROW / 16, KPI = 64 / CPR;  // bytes and 16-byte chunks of a row, keys of an LDS-DMA instruction

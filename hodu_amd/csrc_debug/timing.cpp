@@ -139,6 +139,37 @@ int hodu_rocm_debug_time_product(hodu_rocm_ctx *ctx, int is_matmul, int kind, in
     return time_product_impl(false, ctx, is_matmul, kind, dtype, lhs, rhs_list, n_rhs, out, md, len, iters, elapsed_ms);
 }
 
+int hodu_rocm_debug_record(hodu_rocm_ctx *ctx, int begin, void **graph) {
+    if (!ctx || (!begin && !graph)) return fail(HODU_ROCM_INVALID_ARG, "record: null argument");
+    std::lock_guard<std::recursive_mutex> hold(ctx->mu);
+    HODU_HIP(hipSetDevice(ctx->device));
+    if (begin) {
+        HODU_HIP(hipStreamBeginCapture(ctx->stream, hipStreamCaptureModeThreadLocal));
+        return HODU_ROCM_OK;
+    }
+    hipGraph_t g = nullptr;
+    hipGraphExec_t exec = nullptr;
+    HODU_HIP(hipStreamEndCapture(ctx->stream, &g));
+    const hipError_t e = hipGraphInstantiate(&exec, g, nullptr, nullptr, 0);
+    (void)hipGraphDestroy(g);
+    HODU_HIP(e);
+    *graph = exec;
+    return HODU_ROCM_OK;
+}
+
+int hodu_rocm_debug_replay(hodu_rocm_ctx *ctx, void *graph, int last) {
+    if (!ctx || !graph) return fail(HODU_ROCM_INVALID_ARG, "replay: null argument");
+    std::lock_guard<std::recursive_mutex> hold(ctx->mu);
+    HODU_HIP(hipSetDevice(ctx->device));
+    if (!last) {
+        HODU_HIP(hipGraphLaunch((hipGraphExec_t)graph, ctx->stream));
+        return HODU_ROCM_OK;
+    }
+    HODU_HIP(hipStreamSynchronize(ctx->stream));
+    HODU_HIP(hipGraphExecDestroy((hipGraphExec_t)graph));
+    return HODU_ROCM_OK;
+}
+
 int hodu_rocm_debug_time_product_graph(hodu_rocm_ctx *ctx, int is_matmul, int kind, int dtype, const void *lhs,
                                        const void *const *rhs_list, size_t n_rhs, void *out, const size_t *md,
                                        size_t len, int iters, float *elapsed_ms) {

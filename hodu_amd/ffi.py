@@ -145,6 +145,8 @@ def declare_debug(lib: ctypes.CDLL):
     vpp = ctypes.POINTER(vp)
     lib.hodu_rocm_debug_force_tile.argtypes = [vp, ci]
     lib.hodu_rocm_debug_force_splitk.argtypes = [vp, ci]
+    lib.hodu_rocm_debug_record.argtypes = [vp, ci, vpp]
+    lib.hodu_rocm_debug_replay.argtypes = [vp, vp, ci]
     lib.hodu_rocm_debug_scratch_state.argtypes = [vp, szp, ctypes.POINTER(ci), ctypes.POINTER(ci)]
     lib.hodu_rocm_debug_time_product.argtypes = [vp, ci, ci, ci, vp, vpp, sz, vp, szp, sz, ci, fp]
     lib.hodu_rocm_debug_time_product_graph.argtypes = lib.hodu_rocm_debug_time_product.argtypes
@@ -664,6 +666,17 @@ class Context:
         packed sequences (tiles of 16, 128, 192 or 256 rows), -1 = automatic"""
         self._check(self.debug.hodu_rocm_debug_force_tile(self.handle, int(tile)))
 
+    def record(self, calls) -> "Recording":
+        """testing hook: records what calls() issues on the context's stream instead of running it"""
+        self._check(self.debug.hodu_rocm_debug_record(self.handle, 1, None))
+        graph = ctypes.c_void_p()
+        try:
+            calls()
+        finally:
+            rc = self.debug.hodu_rocm_debug_record(self.handle, 0, ctypes.byref(graph))
+        self._check(rc)
+        return Recording(self, graph)
+
     def force_splitk(self, splits: int):
         """testing hook: K ranges of the pipelined kernels (-1 automatic, 1 never, n forced)"""
         self._check(self.debug.hodu_rocm_debug_force_splitk(self.handle, int(splits)))
@@ -689,6 +702,19 @@ class Context:
     # timing ---------------------------------------------------------------------------------
     def timer(self) -> "Timer":
         return Timer(self)
+
+
+class Recording:
+    """A recorded graph of a context's calls, run in order with its other work."""
+
+    def __init__(self, ctx: Context, graph):
+        self.ctx, self.graph = ctx, graph
+
+    def replay(self):
+        self.ctx._check(self.ctx.debug.hodu_rocm_debug_replay(self.ctx.handle, self.graph, 0))
+
+    def free(self):
+        self.ctx._check(self.ctx.debug.hodu_rocm_debug_replay(self.ctx.handle, self.graph, 1))
 
 
 class Timer:

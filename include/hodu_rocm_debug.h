@@ -25,9 +25,14 @@ extern "C" {
  * variant that cuts K across workgroups wherever it applies, 39 = one block per workgroup with the left operand read
  * in place instead of staged in LDS (what a left operand too large for LDS gets); 40 = the small-product f32 kernel at any size; 41 / 42 / 43 = the f64 matrix-core kernel with
  * 128 x 128 / 64 x 64 / 32 x 32 tiles;
+ * 50 = attention over packed sequences and the paged cache in tiles of 16 rows, 51 = of 128, 52 = of 192 (head dim 128) or 256 (64);
  * -1 = automatic) so that every compiled variant
  * can be exercised at small sizes */
 int hodu_rocm_debug_force_tile(hodu_rocm_ctx *ctx, int tile);
+/* testing hook: begin = 1 starts recording the context's stream into a graph, begin = 0 ends that and hands the graph out;
+ * replay launches it on that stream, with last = 1 waits for the stream and destroys it instead */
+int hodu_rocm_debug_record(hodu_rocm_ctx *ctx, int begin, void **graph);
+int hodu_rocm_debug_replay(hodu_rocm_ctx *ctx, void *graph, int last);
 /* testing hook: what the context itself has allocated for its kernels' scratch -- bytes of its partial-sum workspace
  * (0 = never allocated), whether its arrival counters exist -- and whether it is (still) pointed at the static
  * scratch of the entry point that allocates nothing, which must never be the case between calls */

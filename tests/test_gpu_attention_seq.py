@@ -222,6 +222,22 @@ def test_keys_cut_across_workgroups(ctx, tile, dt, cache_dt, d):
         ctx.force_tile(-1)
 
 
+def test_pages_further_apart_than_32_bits(ctx):
+    """a page stride that the wide kernels' offsets do not hold: the rows go to the other kernel"""
+    q, kc, vc, out, off, table, lens = (ctx.alloc(n) for n in (40 * 4 * 64 * 2, 48 * 2 * 64 * 2, 48 * 2 * 64 * 2, 40 * 4 * 64 * 2, 8, 4, 4))
+    for b in (q, kc, vc):
+        ctx.upload_into(b, np.full(b.nbytes // 2, 0x3F80, np.uint16))
+    ctx.upload_into(off, np.array([0, 40], np.int32))
+    ctx.upload_into(table, np.array([0], np.int32))
+    ctx.upload_into(lens, np.array([48], np.int32))
+    for page, kernel in ((1 << 31, "r16"), (48 * 2 * 64, "wide")):
+        ctx.fill(out, 0xFF)
+        ctx.attention_paged("bf16", q, kc, vc, out, off, table, lens, ffi.paged_attention_md(1, 40, 4, 2, 64, 1, 48, 1, k_cache_strides=(page, 128, 64), v_cache_strides=(page, 128, 64)),
+                            S.scalar(64, "bf16")[0])
+        assert kernel in ctx.last_kernel()
+        assert np.all(ctx.download(out, np.uint16) == 0x3F80)  # the mean of ones
+
+
 def test_many_sequences(ctx):
     """more than a workgroup looks at in one step of its search"""
     g = np.random.default_rng(3)
