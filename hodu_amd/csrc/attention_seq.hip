@@ -506,6 +506,20 @@ template <int D, bool F8, bool PAGED> struct WGeom : SeqGeom<D, F8> {
     static constexpr int LDS = TABLE_AT + (PAGED ? W_WINDOW * 4 : 0);
 };
 
+// lds_get_tr of an address that stays one of LDS for the compiler, which then adds its constant parts in the instruction
+typedef char __attribute__((address_space(3))) * lds_bytes_t;
+template <int SB> __device__ __forceinline__ u32x2_t lds_transpose(lds_bytes_t at) {
+    if constexpr (SB == 2) {
+        typedef short s16x4_t __attribute__((ext_vector_type(4)));
+        typedef s16x4_t __attribute__((address_space(3))) * lds_ptr_t;
+        return __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr_t)at));
+    } else {
+        typedef int i32x2_t __attribute__((ext_vector_type(2)));
+        typedef i32x2_t __attribute__((address_space(3))) * lds_ptr_t;
+        return __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_ptr_t)at));
+    }
+}
+
 template <int CK, int D, bool PAGED, bool F8, int RT>
 __global__ __launch_bounds__(W_NT, 1) void seq_attention_wide_kernel(const uint16_t *__restrict__ Q, const char *__restrict__ K,
                                                                      const char *__restrict__ V, uint16_t *__restrict__ O, DevSeq a,
@@ -627,7 +641,10 @@ __global__ __launch_bounds__(W_NT, 1) void seq_attention_wide_kernel(const uint1
 
     acc_t o[RT][DT + 1];           // the last tile: the row sums
     float e_ref[RT], top[RT];      // exponent reference, the lane's largest new score
-    const u32x4_t one = ones<CK>();
+    float lowest = -INFINITY;
+    mfma::pin_vector(lowest);  // (one instruction for a row's first two scores: as a constant it would vanish, and leave three)
+    u32x4_t one = ones<CK>();
+    mfma::pin_vector(one);  // (or the compiler makes it anew in every step)
 #pragma unroll
     for (int x = 0; x < RT; x++) {
 #pragma unroll
@@ -641,6 +658,7 @@ __global__ __launch_bounds__(W_NT, 1) void seq_attention_wide_kernel(const uint1
     u32x2_t vf[DT * VR];
     const int k_lane = G::k_lane(r, g);
     int v_lane[G::VB];
+    lds_bytes_t v_from[G::VB];
 #pragma unroll
     for (int b2 = 0; b2 < G::VB; b2++) v_lane[b2] = G::V_AT + G::v_lane(r, g, b2);
     auto read_k = [&](int q, int at) __attribute__((always_inline)) {
@@ -653,8 +671,12 @@ __global__ __launch_bounds__(W_NT, 1) void seq_attention_wide_kernel(const uint1
         else return kf[q];
     };
     auto read_v = [&](int q, int at) __attribute__((always_inline)) {
-        const int j = q / VR, from = v_lane[j % G::VB] + at + j / G::VB * G::V_STEP + q % VR * G::V_HALF;
-        vf[q] = lds_get_tr<F8 ? 1 : 2>(smem, from);
+        const int j = q / VR;
+        if (q % VR == 0 && j < G::VB) {
+            v_from[j] = (lds_bytes_t)smem + v_lane[j] + at;
+            mfma::pin_vector(v_from[j]);  // (one register, and what is added to it below an immediate)
+        }
+        vf[q] = lds_transpose<F8 ? 1 : 2>(v_from[j % G::VB] + j / G::VB * G::V_STEP + q % VR * G::V_HALF);
     };
     auto v_operand = [&](int j) __attribute__((always_inline)) -> u32x4_t {
         if constexpr (F8) return widen8<CK>(vf[j]);
@@ -663,11 +685,13 @@ __global__ __launch_bounds__(W_NT, 1) void seq_attention_wide_kernel(const uint1
     // scores of step i beyond what a row attends; the lane's keys are 8 g + 4 t + e
     auto mask = [&](acc_t (&sc)[RT][2], int i) __attribute__((always_inline)) {
 #pragma unroll
-        for (int x = 0; x < RT; x++)
+        for (int x = 0; x < RT; x++) {
+            const int left = open[x] - (i * 32 + 8 * g);
 #pragma unroll
             for (int t = 0; t < 2; t++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) sc[x][t][e] = i * 32 + 8 * g + 4 * t + e < open[x] ? sc[x][t][e] : -INFINITY;
+                for (int e = 0; e < 4; e++) sc[x][t][e] = 4 * t + e < left ? sc[x][t][e] : -INFINITY;
+        }
     };
     auto largest = [&](const acc_t (&sc)[RT][2]) __attribute__((always_inline)) {
 #pragma unroll
@@ -714,7 +738,7 @@ __global__ __launch_bounds__(W_NT, 1) void seq_attention_wide_kernel(const uint1
     auto some_exceed = [&]() __attribute__((always_inline)) {
         bool up = false;
 #pragma unroll
-        for (int x = 0; x < RT; x++) up = up || c * top[x] > e_ref[x] + SLACK;
+        for (int x = 0; x < RT; x++) up |= c * top[x] > e_ref[x] + SLACK;
         return __builtin_amdgcn_ballot_w64(up) != 0;
     };
     // element t (of 8 RT) of a step's exponentials
@@ -791,7 +815,7 @@ __global__ __launch_bounds__(W_NT, 1) void seq_attention_wide_kernel(const uint1
 #pragma unroll
                 for (int w = 0; w < MPC; w++) {
                     const int at = (u - FROM) * MPC + w, x = at >> 3, e = at & 7;
-                    if (at < EL) top[x] = e == 0 ? sn[x][0][0] : __builtin_fmaxf(top[x], sn[x][e >> 2][e & 3]);
+                    if (at < EL) top[x] = __builtin_fmaxf(e == 0 ? lowest : top[x], sn[x][e >> 2][e & 3]);
                 }
                 const int x = ((u - FROM) * MPC + MPC - 1) >> 3;
                 if (x < RT) mfma::pin_vector(top[x]);
