@@ -171,6 +171,9 @@ template <int CK> __device__ __forceinline__ u32x4_t widen8(const u32x2_t &v) {
 // rows; the keys of a tile are cut into ranges of 32-key blocks, one per wavefront of each of the tile's workgroups, so that a single long
 // sequence still reaches every compute unit.  A wavefront has an LDS ring of its own (32 KB: the next block or blocks are in flight while it computes,
 // 64 KB and more per compute unit), meets nobody until its range is done, and there is no barrier in the loop.
+// Measured, bf16, 32 query and 8 key / value heads of 128: 64 tokens over up to 8192 cached each, 1.44 GB, 253 us (5.7 TB/s; a
+// large copy 5.1, reading alone 7.0); 48 over up to 16384 in 8-bit floats, 64 query heads, 1.08 GB, 230 us (4.7 TB/s: what a workgroup
+// costs besides its keys, three rounds of it; eight wavefronts with half the ring each 227); one over 1999, 8 MB, 10.6 us.
 //
 // S^T = K Q^T and O^T += V^T P^T on 16 x 16 x 32: a lane then owns one row throughout (column lane % 16).  The rows
 // of the first product's left operand are keys in the order 8 (r / 4) + 4 t + r % 4 for tile t of two, so that a lane's
@@ -485,6 +488,9 @@ __global__ __launch_bounds__(R16_NT) void seq_attention_r16_kernel(const uint16_
 // rows each (RT = 2, 3 or 4 tiles of 16) and walk all keys of the tile, 64 to a stage of the LDS ring, 32 to a step, with the layouts of the
 // kernel above.  A fragment of K or V read from LDS feeds RT matrix instructions, which is what keeps LDS from being the bound
 // (128 bytes a cycle: a fragment per 2 RT cycles of each SIMD; the instruction takes 16).
+// Measured, bf16, causal, 32 query and 8 key / value heads of 128: 8192 tokens 543 us (1012 TFLOP/s; a matrix product of 8192^3 runs
+// at 1210); 16 prompts of up to 2048 tokens 382 us (642: a workgroup costs some 10 us besides its stages of 1.5 us, and a tile of
+// those has 10 of them); four chunks of 512 tokens over up to 8192 287 us (753).
 //
 // A wavefront issues in order, an instruction every 4 cycles, and a matrix instruction runs for 16: the exponentials have
 // to stand BETWEEN the matrix instructions.  So a step holds three independent pieces of work -- scores of step i + 1,
@@ -1095,7 +1101,9 @@ int launch_seq_attention(hodu_rocm_ctx *ctx, int dtype, int cache_dtype, const v
     };
     // What a launch of wide tiles takes, in ns: a compute unit works on one at a time, so whole rounds of (what a workgroup costs however
     // short it is, what meeting adds, its stages).  Few tiles over a long cache fill the rounds by cutting the keys; the workspace
-    // bounds that at four workgroups per compute unit.
+    // bounds that at four workgroups per compute unit.  Over 4096 cached tokens, head dim 128, whole keys against cut ones: one
+    // chunk of 64 tokens 101 and 31 us, of 256 107 and 40, of 512 112 and 63, of 1024 (a workgroup per unit already: not cut) 127 and 118;
+    // 128 rows against 192: one chunk of 64 31 and 40 us, four of 512 209 and 222, 64 prompts of 128 102 and 86, one of 4096 185 and 180.
     const long keys = g.paged ? (long)a.width * a.page.d : g.k_tokens / sequences, max_stages = (keys + W_BK - 1) / W_BK;
     struct Wide { int rows, splits; long ns; };
     auto wide = [&](int rows, long stage_ns) {
@@ -1118,6 +1126,8 @@ int launch_seq_attention(hodu_rocm_ctx *ctx, int dtype, int cache_dtype, const v
         const int pin = ctx->force_tile;  // testing hook: 50 tiles of 16 rows, 51 of 128, 52 of 192 or 256
         constexpr int BIG = 64 * W_TILES<D>;
         const Wide small = wide(128, D == 128 ? 1400 : 950), big = wide(BIG, D == 128 ? 1750 : 1450);
+        // from three tiles of 16 rows on (over 4096 cached tokens, head dim 128, 16 rows against 128: 4 requests of 8 tokens (32 rows) 34.5
+        // and 31.9 us, of 16 41.5 and 32.1; 16 of 8 59.3 and 59.0, of 16 99 and 60; 64 prompts of 8 tokens 16.8 and 20.1, of 12 23.7 and 20.8)
         const bool wide_rows = avg_rows > 2 * R16;
         if (near && (pin == 52 || (pin < 50 && wide_rows && big.ns < small.ns)))
             return launch(seq_attention_wide_kernel<CK, D, PAGED, F8, W_TILES<D>>, BIG, D, big.splits, WGeom<D, F8, PAGED>::LDS,

@@ -12,7 +12,9 @@ namespace {
 // hundred requests at most times and up to a million slots (4 bytes each, which is what it has to write): every workgroup makes the
 // sums for itself in LDS and then takes its share of the slots, so that nothing has to pass between workgroups and one launch
 // does it.  A token's page comes from the sums (an entry that was in the table before, or the free list's), never from what
-// another workgroup may be writing.  Bound by latency: two trips to memory and a few barriers, then the slots.
+// another workgroup may be writing.  Bound by latency: two trips to memory and a few barriers, then the slots: 8 requests of a token
+// each 4.4 us (of which a launch that does nothing is 1.8), 512 prompts of 700 000 tokens in all 8.3 us.  Running sums by halving
+// strides through LDS, a barrier each, took 19 us for the latter: a wavefront sums by itself, four sums meet at one barrier.
 //
 // The sums saturate at 2^32 - 1 (a saturating sum of non-negative numbers does not depend on its order), which is beyond any
 // list or capacity; who is refused is refused in order, so that what was dealt out is where the first refused request stood.
@@ -160,6 +162,9 @@ __global__ __launch_bounds__(PLAN_NT) void paged_plan_kernel(const int *__restri
 
 // ---- new keys and values into their slots ----------------------------------------------------------------------------
 // One copy: a thread moves 8 elements of a head (16 bytes read; 16 or, as 8-bit floats, 8 written) of k and of v.  Bound by memory.
+// cache[slot] = k or k / scale: 16 bytes of k and of v per thread and turn, neighbouring threads on neighbouring bytes of a head.
+// Bound by memory: 16384 tokens of 8 heads of 128 out of a joint projection into an 8-bit cache, 101 MB, 20 us under the profiler, 5.0 TB/s (a
+// copy of 1 GB: 5.1).  A full division for each element took 23.6 us, the division of an index by a 64-bit one among it.
 struct DevStore {
     int tokens, n_slots;
     long k_token, k_head, v_token, v_head;

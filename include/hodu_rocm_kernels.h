@@ -320,7 +320,9 @@ int hodu_rocm_paged_store(hodu_rocm_ctx *ctx, int dtype, int cache_dtype, const 
  * h / (heads / kv_heads).  causal != 0: row i of n rows over m keys attends keys 0 .. i + m - n (the last row all of
  * them).  A row that attends no key is zero; rows of out behind the last sequence are left as they were; offsets are
  * clamped to the packed lengths.  Scores, softmax and the sums over keys are f32; the probabilities are rounded to
- * `dtype` as the second product's operand and the result once.  out: contiguous [q_tokens, heads, D].
+ * `dtype` as the second product's operand and the result once.  out: contiguous [q_tokens, heads, D].  A key that a row
+ * does not attend has no part in the row, whatever it is; a VALUE of the row's own sequence that is not finite may make
+ * the row NaN although the row does not attend it (zero times infinity), values of other sequences never do.
  * dtype: bf16 or f16; D = 64 or 128; the D elements dense, strides and offsets multiples of 8 elements, bases of 16
  * bytes; scale: the scalar in `dtype`, positive and finite.  HODU_ROCM_UNSUPPORTED otherwise.
  * metadata: [batch, q_tokens, k_tokens, heads, kv_heads, D, q_token, q_head, k_token, k_head, v_token, v_head, q_off,
@@ -339,7 +341,8 @@ int hodu_rocm_attention_varlen(hodu_rocm_ctx *ctx, int dtype, const void *q, con
  * metadata: [batch, q_tokens, heads, kv_heads, D, n_pages, page_size, width, q_token, q_head, q_off, k cache strides
  * (page, token, head), v cache strides (page, token, head), k_cache_off, v_cache_off]; table is [batch, width].
  * Calls with few rows over long contexts cut the keys into ranges and keep partial results in the context's workspace,
- * which may have to grow: run such a call once before capturing it. */
+ * which may have to grow: run such a call once before capturing it, the one with most rows first (a graph keeps the workspace
+ * it was captured with), and replay graphs captured from one context one after the other. */
 int hodu_rocm_attention_paged(hodu_rocm_ctx *ctx, int dtype, int cache_dtype, const void *q, const void *k_cache,
                               const void *v_cache, void *out, const int *q_offsets, const int *table, const int *lens,
                               const float *k_scale, const float *v_scale, const size_t *metadata, size_t metadata_len,

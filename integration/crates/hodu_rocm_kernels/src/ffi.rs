@@ -71,6 +71,23 @@ extern "C" {
                                       scale: *const c_void, causal: c_int, mask: *const c_void, mask_dtype: c_int,
                                       mask_layout: *const usize, mask_layout_len: usize) -> c_int;
 
+    // requests of different lengths: a paged key / value cache and attention over packed sequences
+    pub fn hodu_rocm_paged_plan(ctx: *mut hodu_rocm_ctx, cached: *const c_int, added: *const c_int, free_pages: *const c_int,
+                                table: *mut c_int, lens: *mut c_int, offsets: *mut c_int, slots: *mut c_int, used: *mut c_int,
+                                metadata: *const usize, metadata_len: usize) -> c_int;
+    pub fn hodu_rocm_paged_store(ctx: *mut hodu_rocm_ctx, dtype: c_int, cache_dtype: c_int, k: *const c_void, v: *const c_void,
+                                 k_cache: *mut c_void, v_cache: *mut c_void, slots: *const c_int, k_scale: *const f32,
+                                 v_scale: *const f32, metadata: *const usize, metadata_len: usize) -> c_int;
+    pub fn hodu_rocm_attention_varlen(ctx: *mut hodu_rocm_ctx, dtype: c_int, q: *const c_void, k: *const c_void,
+                                      v: *const c_void, out: *mut c_void, q_offsets: *const c_int, k_offsets: *const c_int,
+                                      metadata: *const usize, metadata_len: usize, scale: *const c_void,
+                                      causal: c_int) -> c_int;
+    pub fn hodu_rocm_attention_paged(ctx: *mut hodu_rocm_ctx, dtype: c_int, cache_dtype: c_int, q: *const c_void,
+                                     k_cache: *const c_void, v_cache: *const c_void, out: *mut c_void,
+                                     q_offsets: *const c_int, table: *const c_int, lens: *const c_int, k_scale: *const f32,
+                                     v_scale: *const f32, metadata: *const usize, metadata_len: usize,
+                                     scale: *const c_void) -> c_int;
+
     // deferred casts fused into the product: bf16 x f8e4m3 bytes -> bf16, i8 x i8 -> i32
     pub fn hodu_rocm_matmul_bf16_f8e4m3w(ctx: *mut hodu_rocm_ctx, lhs: *const c_void, rhs: *const c_void, out: *mut c_void,
                                          metadata: *const usize, metadata_len: usize) -> c_int;

@@ -18,8 +18,8 @@ ALL = os.environ.get("HODU_EMU_ALL", "0") not in ("", "0")
 # {test: the parameters of the cases that run by default}
 HEAVY = {"many_sequences": [], "every_tile": [], "tables_longer_than_what_a_workgroup_holds_of_them": [], "chunks_over_the_cache": [], "longer_prompts": [],
          "scores_that_grow_along_the_keys": [], "prompt_layouts": [], "cache_layouts": [], "calls_in_a_row_give_the_same_bits": [],
-         "keys_cut_across_workgroups": [[51, "bf16", "f8e4m3", 64]], "single_tokens_over_the_cache": [["bf16", "bf16", 64]],
-         "packed_prompts": [["f16", 128, True], ["bf16", 64, False]]}
+         "keys_cut_across_workgroups": [["bf16", "f8e4m3", 64, 51]], "single_tokens_over_the_cache": [[64, "bf16", "bf16"]],
+         "packed_prompts": [[True, 128, "f16"], [False, 64, "bf16"]]}
 
 
 def _cases():
