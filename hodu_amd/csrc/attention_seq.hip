@@ -379,7 +379,17 @@ __global__ __launch_bounds__(R16_NT) void seq_attention_r16_kernel(const uint16_
 #pragma unroll
         for (int e = 0; e < 8; e++) p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[e], c, -e_ref));
         const u32x4_t pf = {pack2<CK>(p[0], p[1]), pack2<CK>(p[2], p[3]), pack2<CK>(p[4], p[5]), pack2<CK>(p[6], p[7])};
+        // What P's rounding left is multiplied too, as a second operand: a single token's output is then as exact as its own rounding (the
+        // matrix instructions are not the bound here; with P rounded once the error was 1.4 times that).
+        float rest[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const uint16_t w = (uint16_t)(pf[e >> 1] >> (16 * (e & 1)));
+            rest[e] = p[e] - (F16 ? f16_bits_to_f32(w) : bf16_bits_to_f32(w));
+        }
+        const u32x4_t pr = {pack2<CK>(rest[0], rest[1]), pack2<CK>(rest[2], rest[3]), pack2<CK>(rest[4], rest[5]), pack2<CK>(rest[6], rest[7])};
         Cmp::mma(one, pf, o[G::DT]);
+        Cmp::mma(one, pr, o[G::DT]);
 #pragma unroll
         for (int j = 0; j < G::DT; j++) {
             const int at = v_lane[j % G::VB] + j / G::VB * G::V_STEP;
@@ -391,6 +401,7 @@ __global__ __launch_bounds__(R16_NT) void seq_attention_r16_kernel(const uint16_
                 vf = u32x4_t{lo.x, lo.y, hi.x, hi.y};
             }
             Cmp::mma(vf, pf, o[j]);
+            Cmp::mma(vf, pr, o[j]);
         }
         if (blk + G::RING < blk1) {
             // the block's reads have been answered before its slot's next loads are issued
