@@ -304,7 +304,10 @@ class DeviceView:
 
     @classmethod
     def of(cls, tensor) -> "DeviceView":
-        """of a torch tensor: its elements or, where they do not lie side by side, all up to the end of its storage"""
+        """of a torch tensor on the context's device: its elements or, where they do not lie side by side, all up to the end of its
+        storage"""
+        if not tensor.is_cuda:
+            raise ValueError(f"a tensor on the GPU is needed, got one on {tensor.device}")
         if tensor.is_contiguous():
             return cls(tensor.data_ptr(), tensor.nbytes)
         return cls(tensor.data_ptr(), tensor.untyped_storage().nbytes() - tensor.storage_offset() * tensor.element_size())
