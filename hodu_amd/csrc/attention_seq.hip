@@ -112,7 +112,9 @@ template <int ROWS, bool PAGED> __device__ __forceinline__ bool find_tile(const 
 }
 
 // The same for tiles that work for long, of up to 64 sequences: the ones with most keys first and each from its last row, so that
-// the tiles left over at a launch's end are short ones.  A lane owns a sequence, sums the tiles of those before it in that order, and
+// the tiles left over at a launch's end are short ones (in the sequences' own order and with it: 8192 tokens 679 and 594 us, four chunks of
+// 512 over up to 8192 390 and 361, 64 single tokens over up to 8192 270 and 254, 16 packed prompts 421 and 413).  Above 64, one sequence a
+// lane does not do, and a launch has rounds enough to even out.  A lane owns a sequence, sums the tiles of those before it in that order, and
 // knows whether the tile is its own.
 template <int ROWS, bool PAGED> __device__ __forceinline__ bool find_tile_long_first(const DevSeq &a, int tile, SeqTile &f) {
     const int lane = threadIdx.x & 63, s = lane < a.batch ? lane : a.batch - 1;
