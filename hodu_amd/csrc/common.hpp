@@ -4,6 +4,7 @@
 #include <hip/hip_runtime.h>
 
 #include <mutex>
+#include <vector>
 
 #include <cstddef>
 #include <cstdint>
@@ -20,6 +21,7 @@ namespace hodu {
 struct Workspace {
     void *ptr = nullptr;
     size_t bytes = 0;
+    bool recorded = false;  // a call that was captured into a graph took it: replays write to it, whatever the context does since
 };
 
 }  // namespace hodu
@@ -29,6 +31,7 @@ struct hodu_rocm_ctx {
     hipStream_t stream = nullptr;
     hipDeviceProp_t props{};
     hodu::Workspace workspace;  // split-K partial sums; grown on demand, owned by the context
+    std::vector<void *> outgrown;  // workspaces that a graph may still write to: freed with the context
     int *arrival = nullptr;     // kArrivalSlots zeroed counters for kernels whose last workgroup finishes a reduction
     // The counters `arrival` points at may hold something other than zeros (fresh memory; a launch that failed part
     // way; the shared static array, which keeps what the last call on this GPU left): ensure_arrival zeroes them, by
@@ -84,7 +87,8 @@ inline int ensure_dynamic_lds(hodu_rocm_ctx *ctx, const void *kernel, int bytes)
 }
 
 // grows ctx->workspace to at least `bytes` (refused, with an error text, while ctx->fixed_scratch is set and the
-// static scratch is smaller, or while the context's stream is being captured into a graph and it would have to grow)
+// static scratch is smaller, or while the context's stream is being captured into a graph and it would have to grow).
+// A block that a captured call took is kept when the workspace outgrows it: graphs hold its address.
 int ensure_workspace(hodu_rocm_ctx *ctx, size_t bytes);
 // allocates ctx->arrival (once) and zeroes the counters whenever ctx->arrival_stale says they may not be zero; a
 // kernel that uses a counter leaves it at zero again, so a launch that runs to completion keeps them clean.  Every

@@ -1,6 +1,7 @@
 // Context, memory and timing entry points of the C ABI.
 #include <cstdarg>
 #include <cstring>
+#include <new>
 
 #include "common.hpp"
 
@@ -65,7 +66,10 @@ bool stream_is_capturing(hipStream_t s) {
 }  // namespace
 
 int ensure_workspace(hodu_rocm_ctx *ctx, size_t bytes) {
-    if (ctx->workspace.bytes >= bytes) return HODU_ROCM_OK;
+    if (ctx->workspace.bytes >= bytes) {
+        if (!ctx->fixed_scratch && !ctx->workspace.recorded && stream_is_capturing(ctx->stream)) ctx->workspace.recorded = true;
+        return HODU_ROCM_OK;
+    }
     if (ctx->fixed_scratch)
         return fail(HODU_ROCM_SCRATCH,
                     "this product needs %zu bytes of partial sums; the static scratch of the entry point that "
@@ -73,7 +77,14 @@ int ensure_workspace(hodu_rocm_ctx *ctx, size_t bytes) {
     if (stream_is_capturing(ctx->stream))
         return fail(HODU_ROCM_SCRATCH, "the workspace would have to grow to %zu bytes while the stream is being "
                     "captured: run the product once outside the capture first", bytes);
-    if (ctx->workspace.ptr) {
+    if (ctx->workspace.recorded) {
+        try {
+            ctx->outgrown.push_back(ctx->workspace.ptr);
+        } catch (const std::bad_alloc &) {
+            return fail(HODU_ROCM_OOM, "no host memory to keep track of a workspace that a graph holds");
+        }
+        ctx->workspace = Workspace();
+    } else if (ctx->workspace.ptr) {
         HODU_HIP(hipStreamSynchronize(ctx->stream));
         HODU_HIP(hipFree(ctx->workspace.ptr));
         ctx->workspace = Workspace();
@@ -165,6 +176,7 @@ int hodu_rocm_ctx_destroy(hodu_rocm_ctx *ctx) {
     (void)hipSetDevice(ctx->device);
     (void)hipStreamSynchronize(ctx->stream);
     if (ctx->workspace.ptr) (void)hipFree(ctx->workspace.ptr);
+    for (void *p : ctx->outgrown) (void)hipFree(p);
     if (ctx->arrival) (void)hipFree(ctx->arrival);
     (void)hipStreamDestroy(ctx->stream);
     delete ctx;

@@ -341,8 +341,10 @@ int hodu_rocm_attention_varlen(hodu_rocm_ctx *ctx, int dtype, const void *q, con
  * metadata: [batch, q_tokens, heads, kv_heads, D, n_pages, page_size, width, q_token, q_head, q_off, k cache strides
  * (page, token, head), v cache strides (page, token, head), k_cache_off, v_cache_off]; table is [batch, width].
  * Calls with few rows over long contexts cut the keys into ranges and keep partial results in the context's workspace,
- * which may have to grow: run such a call once before capturing it, the one with most rows first (a graph keeps the workspace
- * it was captured with), and replay graphs captured from one context one after the other. */
+ * which may have to grow (not with the rows: fewer of them are cut into more ranges).  It cannot grow while the stream is
+ * being captured -- such a call is refused with HODU_ROCM_SCRATCH: run it once, with the same sizes, before capturing it.
+ * A graph keeps the workspace it was captured with for as long as the context lives, also when later calls need a larger
+ * one; replay graphs captured from one context one after the other. */
 int hodu_rocm_attention_paged(hodu_rocm_ctx *ctx, int dtype, int cache_dtype, const void *q, const void *k_cache,
                               const void *v_cache, void *out, const int *q_offsets, const int *table, const int *lens,
                               const float *k_scale, const float *v_scale, const size_t *metadata, size_t metadata_len,

@@ -117,6 +117,11 @@ const char *emu_last_error(void) { return hodu::get_error(); }
 void emu_lds_fill(int byte) { memset(emu::lds_base(), byte, emu::kLdsBytes); }
 // where an allocation touches its guard page: 1 its end (the default), 0 its start
 void emu_alloc_tight(int end) { emu::g_tight_end = end != 0; }
+// "device" allocations that have not been freed
+int emu_live_allocations(void) {
+    std::lock_guard<std::mutex> hold(emu::g_alloc_mu);
+    return (int)emu::g_allocs.size();
+}
 // how often a kernel reached an instruction that has no CPU stand-in (must stay 0 for a result to mean anything)
 int emu_unsupported_hits(void) { return emu::no_such_instruction_hits(); }
 const char *emu_unsupported_first(void) { return emu::no_such_instruction_first(); }
