@@ -28,7 +28,9 @@ struct Workspace {
 
 struct hodu_rocm_ctx {
     int device = 0;
-    hipStream_t stream = nullptr;
+    hipStream_t stream = nullptr;      // what every call is issued on: own_stream, or the caller's
+    hipStream_t own_stream = nullptr;  // created and destroyed with the context
+    hipEvent_t handover = nullptr;     // orders a new stream behind the one before it
     hipDeviceProp_t props{};
     hodu::Workspace workspace;  // split-K partial sums; grown on demand, owned by the context
     std::vector<void *> outgrown;  // workspaces that a graph may still write to: freed with the context

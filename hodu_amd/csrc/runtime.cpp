@@ -60,7 +60,11 @@ __global__ __launch_bounds__(1024) void clear_words_kernel(int *__restrict__ p, 
 
 bool stream_is_capturing(hipStream_t s) {
     hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
-    return hipStreamIsCapturing(s, &st) == hipSuccess && st != hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(s, &st) != hipSuccess) {
+        (void)hipGetLastError();  // (the default stream, while another one is captured: no error of the call at hand)
+        return false;
+    }
+    return st != hipStreamCaptureStatusNone;
 }
 
 }  // namespace
@@ -147,7 +151,12 @@ int hodu_rocm_ctx_create(int device, hodu_rocm_ctx **out) {
     hodu_rocm_ctx *ctx = new hodu_rocm_ctx();
     ctx->device = device;
     hipError_t e = hipGetDeviceProperties(&ctx->props, device);
-    if (e == hipSuccess) e = hipStreamCreateWithFlags(&ctx->stream, hipStreamNonBlocking);
+    if (e == hipSuccess) e = hipStreamCreateWithFlags(&ctx->own_stream, hipStreamNonBlocking);
+    if (e == hipSuccess) {
+        e = hipEventCreateWithFlags(&ctx->handover, hipEventDisableTiming);
+        if (e != hipSuccess) (void)hipStreamDestroy(ctx->own_stream);
+    }
+    ctx->stream = ctx->own_stream;
     if (e != hipSuccess) {
         delete ctx;
         return fail(HODU_ROCM_HIP_ERROR, "context setup: %s", hipGetErrorString(e));
@@ -156,14 +165,16 @@ int hodu_rocm_ctx_create(int device, hodu_rocm_ctx **out) {
         // the embedded code object is gfx950 only; any launch would fail with a less clear error
         char arch[64];
         snprintf(arch, sizeof(arch), "%s", ctx->props.gcnArchName);
-        (void)hipStreamDestroy(ctx->stream);
+        (void)hipEventDestroy(ctx->handover);
+        (void)hipStreamDestroy(ctx->own_stream);
         delete ctx;
         return fail(HODU_ROCM_UNSUPPORTED, "device %d is %s; this library carries gfx950 code only", device, arch);
     }
     // this device's address of the static scratch array (the device is current): kept for the entry point that
     // allocates nothing
     if (int rc = static_scratch_of(device, &ctx->static_scratch)) {
-        (void)hipStreamDestroy(ctx->stream);
+        (void)hipEventDestroy(ctx->handover);
+        (void)hipStreamDestroy(ctx->own_stream);
         delete ctx;
         return rc;
     }
@@ -174,12 +185,44 @@ int hodu_rocm_ctx_create(int device, hodu_rocm_ctx **out) {
 int hodu_rocm_ctx_destroy(hodu_rocm_ctx *ctx) {
     if (!ctx) return HODU_ROCM_OK;
     (void)hipSetDevice(ctx->device);
-    (void)hipStreamSynchronize(ctx->stream);
+    // (a caller's stream may be gone by now: the device is waited for, and the stream not touched)
+    if (ctx->stream == ctx->own_stream) (void)hipStreamSynchronize(ctx->stream);
+    else (void)hipDeviceSynchronize();
     if (ctx->workspace.ptr) (void)hipFree(ctx->workspace.ptr);
     for (void *p : ctx->outgrown) (void)hipFree(p);
     if (ctx->arrival) (void)hipFree(ctx->arrival);
-    (void)hipStreamDestroy(ctx->stream);
+    (void)hipEventDestroy(ctx->handover);
+    (void)hipStreamDestroy(ctx->own_stream);
     delete ctx;
+    return HODU_ROCM_OK;
+}
+
+int hodu_rocm_ctx_stream(hodu_rocm_ctx *ctx, void **stream) {
+    clear_error();
+    if (!ctx || !stream) return fail(HODU_ROCM_INVALID_ARG, "ctx_stream: null argument");
+    std::lock_guard<std::recursive_mutex> hold(ctx->mu);
+    *stream = (void *)ctx->stream;
+    return HODU_ROCM_OK;
+}
+
+int hodu_rocm_ctx_set_stream(hodu_rocm_ctx *ctx, void *stream) {
+    clear_error();
+    REQUIRE_CTX(ctx);
+    std::lock_guard<std::recursive_mutex> hold(ctx->mu);
+    const hipStream_t next = (hipStream_t)stream;
+    if (next == ctx->stream) return HODU_ROCM_OK;
+    if (next) {
+        int device = -1;
+        HODU_HIP(hipStreamGetDevice(next, &device));
+        if (device != ctx->device)
+            return fail(HODU_ROCM_INVALID_ARG, "ctx_set_stream: a stream of device %d for a context on device %d", device, ctx->device);
+    }
+    // (an event crosses neither into a capture nor out of one)
+    if (stream_is_capturing(ctx->stream) || stream_is_capturing(next))
+        return fail(HODU_ROCM_INVALID_ARG, "ctx_set_stream: a stream is being captured: hand it over before the capture begins");
+    HODU_HIP(hipEventRecord(ctx->handover, ctx->stream));
+    HODU_HIP(hipStreamWaitEvent(next, ctx->handover, 0));
+    ctx->stream = next;
     return HODU_ROCM_OK;
 }
 

@@ -85,6 +85,8 @@ def declare_runtime(lib: ctypes.CDLL):
     lib.hodu_rocm_memcpy_d2d.argtypes = [vp, vp, vp, sz]
     lib.hodu_rocm_memset.argtypes = [vp, vp, ci, sz]
     lib.hodu_rocm_sync.argtypes = [vp]
+    lib.hodu_rocm_ctx_stream.argtypes = [vp, ctypes.POINTER(vp)]
+    lib.hodu_rocm_ctx_set_stream.argtypes = [vp, vp]
     lib.hodu_rocm_last_error.argtypes = [vp]
     lib.hodu_rocm_last_error.restype = ctypes.c_char_p
     lib.hodu_rocm_last_kernel.argtypes = [vp]
@@ -295,8 +297,8 @@ class DeviceBuffer:
 
 class DeviceView:
     """Device memory that somebody else owns (another library's tensor, a part of a DeviceBuffer), as an operand: the
-    calls that take a DeviceBuffer take one of these.  The owner keeps the memory alive and orders its own work on it
-    against the context's stream."""
+    calls that take a DeviceBuffer take one of these.  The owner keeps the memory alive, and its own work on it is in order
+    with the context's calls only where they share a stream: Context.set_stream(torch.cuda.current_stream())."""
     __slots__ = ("ptr", "nbytes")
 
     def __init__(self, ptr: int, nbytes: int):
@@ -372,6 +374,25 @@ class Context:
 
     def sync(self):
         self._check(self.lib.hodu_rocm_sync(self.handle))
+
+    # the stream that was handed over last, so that a loop's step that hands over the same one again costs nothing
+    _stream: Optional[int] = None
+
+    @property
+    def stream(self) -> int:
+        """the stream that the context's calls are issued on (a hipStream_t; at first the context's own)"""
+        s = ctypes.c_void_p()
+        self._check(self.lib.hodu_rocm_ctx_stream(self.handle, ctypes.byref(s)))
+        return s.value or 0
+
+    def set_stream(self, stream):
+        """hodu_rocm_ctx_set_stream: issue every later call on `stream` -- a hipStream_t as a number (0: the default stream) or
+        an object that has one as cuda_stream, as torch's streams do -- behind what the context issued before.  The
+        stream has to stay alive until another one is set or the context closed"""
+        handle = int(getattr(stream, "cuda_stream", stream))
+        if handle != self._stream:
+            self._check(self.lib.hodu_rocm_ctx_set_stream(self.handle, handle))
+            self._stream = handle
 
     # compute --------------------------------------------------------------------------------
     def product(self, op: str, name: str, lhs: DeviceBuffer, rhs: DeviceBuffer, out: DeviceBuffer, md):

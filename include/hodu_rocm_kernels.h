@@ -70,6 +70,14 @@ int hodu_rocm_memcpy_d2h(hodu_rocm_ctx *ctx, void *dst_host, const void *src_dev
 int hodu_rocm_memcpy_d2d(hodu_rocm_ctx *ctx, void *dst_device, const void *src_device, size_t bytes);
 int hodu_rocm_memset(hodu_rocm_ctx *ctx, void *dptr, int byte, size_t bytes);
 int hodu_rocm_sync(hodu_rocm_ctx *ctx);
+/* The stream that the context's calls are issued on, a hipStream_t: at first one of its own, which is ordered against no
+ * other, not against the default stream either.  A caller whose operands are written or read by work on a stream of
+ * its own (another library's) hands that stream over, and every later call is in order with that work; NULL is the
+ * default stream.  What was issued before the change runs before anything issued after it.  The stream belongs to the
+ * context's device and stays alive until another one is handed over or the context is destroyed; neither it nor the one before
+ * may be in a capture at that moment (INVALID_ARG): hand a stream over first, then capture it.                       */
+int hodu_rocm_ctx_stream(hodu_rocm_ctx *ctx, void **stream);
+int hodu_rocm_ctx_set_stream(hodu_rocm_ctx *ctx, void *stream);
 /* message of the last failing call made on this context by the calling thread ("" if none) */
 const char *hodu_rocm_last_error(hodu_rocm_ctx *ctx);
 /* device facts for roofline reporting: name (<=255 chars), compute units, clock (kHz), memory bytes */

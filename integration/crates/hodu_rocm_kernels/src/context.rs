@@ -5,7 +5,7 @@ use core::ffi::{c_int, c_void};
 use std::ffi::CStr;
 use std::sync::Arc;
 
-/// One `hodu_rocm_ctx` (one device, one stream).  The library serialises calls on a context internally and never
+/// One `hodu_rocm_ctx` (one device, one stream at a time).  The library serialises calls on a context internally and never
 /// calls back, so sharing it between threads is sound.
 pub struct Context {
     raw: *mut ffi::hodu_rocm_ctx,
@@ -61,6 +61,19 @@ impl Context {
         Ok(out)
     }
     pub fn sync(&self) -> Result<()> { self.check(unsafe { ffi::hodu_rocm_sync(self.raw) }) }
+    /// the stream (a hipStream_t) that the context's calls are issued on; at first one of its own
+    pub fn stream(&self) -> Result<*mut c_void> {
+        let mut s: *mut c_void = core::ptr::null_mut();
+        self.check(unsafe { ffi::hodu_rocm_ctx_stream(self.raw, &mut s) })?;
+        Ok(s)
+    }
+    /// issues every later call on `stream` (null: the default stream), behind what was issued before
+    ///
+    /// # Safety
+    /// `stream` is a hipStream_t of the context's device, alive until another one is set or the context dropped.
+    pub unsafe fn set_stream(&self, stream: *mut c_void) -> Result<()> {
+        self.check(ffi::hodu_rocm_ctx_set_stream(self.raw, stream))
+    }
     /// Products of f8e4m3 / f8e5m2 / bf16 / f16 in the CPU backend's arithmetic (the running sum re-rounded to the dtype
     /// after every multiply and add): byte for byte what `hodu_cpu_matmul_<dt>` stores, at a scalar loop's speed.  For
     /// tests that compare devices bit for bit; off by default.

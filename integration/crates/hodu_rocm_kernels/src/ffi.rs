@@ -46,6 +46,8 @@ extern "C" {
     pub fn hodu_rocm_memcpy_d2h(ctx: *mut hodu_rocm_ctx, dst: *mut c_void, src: *const c_void, bytes: usize) -> c_int;
     pub fn hodu_rocm_memcpy_d2d(ctx: *mut hodu_rocm_ctx, dst: *mut c_void, src: *const c_void, bytes: usize) -> c_int;
     pub fn hodu_rocm_sync(ctx: *mut hodu_rocm_ctx) -> c_int;
+    pub fn hodu_rocm_ctx_stream(ctx: *mut hodu_rocm_ctx, stream: *mut *mut c_void) -> c_int;
+    pub fn hodu_rocm_ctx_set_stream(ctx: *mut hodu_rocm_ctx, stream: *mut c_void) -> c_int;
     pub fn hodu_rocm_last_error(ctx: *mut hodu_rocm_ctx) -> *const c_char;
     pub fn hodu_rocm_ctx_set_reference_sums(ctx: *mut hodu_rocm_ctx, on: c_int) -> c_int;
 

@@ -127,6 +127,8 @@ int emu_unsupported_hits(void) { return emu::no_such_instruction_hits(); }
 const char *emu_unsupported_first(void) { return emu::no_such_instruction_first(); }
 void emu_unsupported_reset(void) { emu::no_such_instruction_hits() = 0; }
 #ifdef EMU_WITH_RUNTIME
+// the last hipStreamWaitEvent: the stream that waits, and the one whose work it waits for
+void emu_last_wait(void **waiter, void **waited_for) { *waiter = emu::last_wait().waiter; *waited_for = emu::last_wait().waited_for; }
 void emu_dma_lazy(int model) { emu::dma_lazy() = model; }
 // the two probes of the debug library that are kernels written around inline assembly (clock_probe.hip) have no CPU build;
 // the rest of it (csrc_debug/timing.cpp: hooks, scratch report, timing loops, graph replay) is compiled as it is

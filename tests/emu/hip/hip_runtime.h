@@ -74,8 +74,10 @@ inline hipError_t hipFuncSetAttribute(const void *, hipFuncAttribute, int) { ret
 inline hipError_t hipGetDeviceCount(int *n) { *n = 1; return hipSuccess; }
 inline hipError_t hipGetDeviceProperties(hipDeviceProp_t *p, int) { *p = hipDeviceProp_t(); return hipSuccess; }
 constexpr unsigned hipStreamNonBlocking = 1;
-inline hipError_t hipStreamCreateWithFlags(hipStream_t *s, unsigned) { *s = nullptr; return hipSuccess; }
-inline hipError_t hipStreamDestroy(hipStream_t) { return hipSuccess; }
+inline hipError_t hipStreamCreateWithFlags(hipStream_t *s, unsigned) { *s = new char; return hipSuccess; }
+inline hipError_t hipStreamDestroy(hipStream_t s) { delete (char *)s; return hipSuccess; }
+inline hipError_t hipStreamGetDevice(hipStream_t, int *device) { *device = 0; return hipSuccess; }
+inline hipError_t hipDeviceSynchronize() { return hipSuccess; }
 inline hipError_t hipStreamSynchronize(hipStream_t) { return hipSuccess; }
 // Graphs: while the (one) stream is being captured, a kernel launch or a memset is recorded instead of run; launching
 // the instantiated graph runs the recorded nodes in order.
@@ -129,10 +131,18 @@ inline hipError_t hipMemsetAsync(void *dst, int byte, size_t bytes, hipStream_t)
 #define HIP_SYMBOL(x) (x)
 template <class T> inline hipError_t hipGetSymbolAddress(void **p, T &symbol) { *p = (void *)&symbol; return hipSuccess; }
 // events: the host's clock at the moment of recording (everything before it on the one stream has run by then)
-struct emu_event { std::chrono::steady_clock::time_point at; };
+struct emu_event { std::chrono::steady_clock::time_point at; hipStream_t on = nullptr; };
 typedef emu_event *hipEvent_t;
-inline hipError_t hipEventCreate(hipEvent_t *e) { *e = new emu_event{std::chrono::steady_clock::now()}; return hipSuccess; }
-inline hipError_t hipEventRecord(hipEvent_t e, hipStream_t) { e->at = std::chrono::steady_clock::now(); return hipSuccess; }
+inline hipError_t hipEventCreate(hipEvent_t *e) { *e = new emu_event{std::chrono::steady_clock::now(), nullptr}; return hipSuccess; }
+constexpr unsigned hipEventDisableTiming = 2;
+inline hipError_t hipEventCreateWithFlags(hipEvent_t *e, unsigned) { return hipEventCreate(e); }
+inline hipError_t hipEventRecord(hipEvent_t e, hipStream_t s) { e->at = std::chrono::steady_clock::now(); e->on = s; return hipSuccess; }
+// (everything runs at once; what a test can see is which stream was told to wait for which)
+namespace emu {
+struct Wait { hipStream_t waiter = nullptr, waited_for = nullptr; };
+inline Wait &last_wait() { static Wait w; return w; }
+}  // namespace emu
+inline hipError_t hipStreamWaitEvent(hipStream_t s, hipEvent_t e, unsigned) { emu::last_wait() = {s, e->on}; return hipSuccess; }
 inline hipError_t hipEventSynchronize(hipEvent_t) { return hipSuccess; }
 inline hipError_t hipEventElapsedTime(float *ms, hipEvent_t a, hipEvent_t b) {
     *ms = std::chrono::duration<float, std::milli>(b->at - a->at).count();
