@@ -1,5 +1,9 @@
 """A context on the stream of the library that owns the operands (torch here): calls in order with that library's work without a
 synchronization between them, eager and captured into its graphs."""
+import importlib.util
+import os
+import random
+
 import numpy as np
 import pytest
 import torch
@@ -8,6 +12,8 @@ from hodu_amd import ffi
 import seq_util as S
 
 pytestmark = pytest.mark.gpu
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
 @pytest.fixture()
@@ -113,3 +119,44 @@ def test_captured_into_the_owners_graph(ctx):
             p.call()  # eager work between the replays
         torch.cuda.synchronize()
         assert torch.equal(p.out, want)
+
+
+def test_the_measured_calls_are_in_order_with_torch():
+    """a pass of perf/operators.py on inputs that are still being made, its outputs taken at once, no synchronization"""
+    spec = importlib.util.spec_from_file_location("measured_operators", os.path.join(ROOT, "perf", "operators.py"))
+    ops = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(ops)
+    cases = [c for c in ops.listed() if c["name"] in ("plan_decode", "store_decode", "prompt_short", "decode_one")]
+    rng = random.Random(5)
+    while len(cases) < 10:
+        c = ops.draw(rng)
+        if ops.work(c)["flops"] < 2e10 and ops.work(c)["bytes"] < 5e7:
+            cases.append(c)
+
+    def values(out):
+        return list(out.values()) if isinstance(out, dict) else [out]
+
+    for n, case in enumerate(cases):
+        plain, late = ops.prepare(case, n), ops.prepare(case, n)
+        given = {k: x.clone() for k, x in late.items() if torch.is_tensor(x) and x.is_cuda}
+        for x in given:
+            late[x].zero_()
+        torch.cuda.synchronize()
+        torch.cuda._sleep(20_000_000)
+        for k, x in given.items():
+            late[k].copy_(x)
+        ops.own = True
+        try:
+            got = [x.clone() for x in values(ops.run(late))]
+        finally:
+            ops.own = False
+        for k in given:
+            late[k].zero_()
+        want = [x.clone() for x in values(ops.run(plain))]
+        for a, b in zip(got, want):
+            if a.dtype == torch.int32 or case["op"] == "store" and case["cache"] != "f8e4m3":
+                assert torch.equal(a, b), case
+            else:
+                x, y = a.double(), b.double()
+                # (roundings of P and of the output, and an 8-bit value next to a tie: far below what stale operands give)
+                assert (x - y).norm() <= 2 * S.HALF_STEP[{v: k for k, v in S.TORCH.items()}[a.dtype]] * y.norm(), case
