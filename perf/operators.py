@@ -307,8 +307,10 @@ def _own(s):
 
     if _context is None:
         _context = ffi.Context(0)
+        # the operands are torch's: the calls are in order with its work on them, before and after (handed over once, as by a
+        # program that stays on the stream it begins with)
+        _context.set_stream(torch.cuda.current_stream())
     c, case, of = _context, s["case"], ffi.DeviceView.of
-    c.set_stream(torch.cuda.current_stream())  # the operands are torch's: in order with its work on them, before and after
     if case["op"] == "plan":
         c.paged_plan(of(s["cached"]), of(s["added"]), of(s["free"]), of(s["table"]), of(s["lens"]), of(s["offsets"]), of(s["slots"]),
                      of(s["used"]), ffi.paged_plan_md(case["batch"], case["page"], s["table"].shape[1], s["free"].shape[0], s["slots"].shape[0]))
