@@ -224,6 +224,14 @@ template <int D, bool F8> struct R16Geom : SeqGeom<D, F8> {
     static constexpr int WINDOW_AT = R16_WAVES * WAVE > MERGE ? R16_WAVES * WAVE : MERGE;
     static constexpr int LDS = WINDOW_AT + R16_WAVES * R16_WINDOW * 4 + 16;
 };
+// How far a score may exceed the exponent reference of its row before the reference moves (as a power of two), and how far above the
+// largest score a new reference is put.  In bf16 by as much: P is at most one, so the sums over the keys reach no further than
+// the sum of the values themselves, which may be as large as f32 holds.  f16 keeps few digits of a P below 2^-14, so there P reaches
+// up to 2^12 instead; its values are below 2^16, and the sums far from f32's end.  Scores that rise by 2^12 over a row's first are
+// rare, and a move of the reference is what a step costs.
+template <int CK> struct Slack {
+    static constexpr float SLACK = 12.f, LIFT = CK == mfma::CK_F16 ? 0.f : SLACK;
+};
 // 1.0 in every element: the row sums are one more tile of the second product, over the P that it multiplies (which is rounded,
 // so that the weights sum to one), and cost no vector instruction and no exchange between a row's lanes
 template <int CK> __device__ __forceinline__ u32x4_t ones() {
@@ -320,7 +328,7 @@ __global__ __launch_bounds__(R16_NT) void seq_attention_r16_kernel(const uint16_
 #pragma unroll
     for (int b = 0; b < G::VB; b++) v_lane[b] = G::v_lane(r, g, b);
     // the exponent reference, an integer that moves only when a score exceeds it by 2^SLACK: see the wide kernel below
-    constexpr float SLACK = F16 ? 12.f : 64.f;
+    constexpr float SLACK = Slack<CK>::SLACK, LIFT = Slack<CK>::LIFT;
     float e_ref = -1e30f;
     if (blk0 < blk1) {
         if constexpr (PAGED) fill_window(quot(blk0 * R16_BK, a.page));
@@ -366,10 +374,10 @@ __global__ __launch_bounds__(R16_NT) void seq_attention_r16_kernel(const uint16_
         float top = sv[0];
 #pragma unroll
         for (int e = 1; e < 8; e++) top = __builtin_fmaxf(top, sv[e]);
-        if (__builtin_amdgcn_ballot_w64(c * top > e_ref + SLACK) != 0) {
+        if (__builtin_amdgcn_ballot_w64(c * top > e_ref + (SLACK - LIFT)) != 0) {
             top = __builtin_fmaxf(top, __shfl_xor(top, 16));
             top = c * __builtin_fmaxf(top, __shfl_xor(top, 32));
-            const float e_new = top > e_ref + SLACK ? ceilf(top) : e_ref;
+            const float e_new = top > e_ref + (SLACK - LIFT) ? ceilf(top) + LIFT : e_ref;
             const float keep = __builtin_amdgcn_exp2f(e_ref - e_new);
             e_ref = e_new;
 #pragma unroll
@@ -511,9 +519,9 @@ __global__ __launch_bounds__(R16_NT) void seq_attention_r16_kernel(const uint16_
 // a share of the vector work and LDS reads in each, which the compiler may not reorder across (sched_barrier, and the empty
 // statements that pin a chunk's results to it).
 //
-// The exponent reference of a row is an integer E >= c max - SLACK, c = scale log2 e: p = 2^(c s - E) <= 2^SLACK (f32 and bf16 reach to 2^127, f16 to 2^16).  It moves only when a
-// score exceeds it by 2^SLACK, which the lanes find out without talking to each other (any lane's own maximum); then the row's lanes
-// agree on the new one and O, the row sum and the P not yet multiplied are rescaled -- by a power of two, exactly.
+// The exponent reference of a row is an integer E, ceil(c max) + LIFT when it was last set, c = scale log2 e; p = 2^(c s - E).  It moves only
+// when a score reaches c s > E + SLACK - LIFT, which the lanes find out without talking to each other (any lane's own maximum); then the
+// row's lanes agree on the new one and O, the row sum and the P not yet multiplied are rescaled -- by a power of two, exactly.
 // Row tiles per wavefront: 3 at head dim 128 (O, q, two steps' scores and P are 84 registers a tile; with 4 the allocator runs out),
 // 4 at 64.
 template <int D> constexpr int W_TILES = D == 128 ? 3 : 4;
@@ -722,7 +730,7 @@ __global__ __launch_bounds__(W_NT, 1) void seq_attention_wide_kernel(const uint1
     };
     // Moves the references of the rows whose new scores exceed them by too much (rare: some lane saw one); pc: the P that is
     // still to be multiplied
-    constexpr float SLACK = F16 ? 12.f : 64.f;
+    constexpr float SLACK = Slack<CK>::SLACK, LIFT = Slack<CK>::LIFT;
     auto move_references = [&](u32x4_t (&pc)[RT]) __attribute__((always_inline)) {
         mfma::mfma_results_settle();
         __builtin_amdgcn_sched_barrier(0);
@@ -730,7 +738,7 @@ __global__ __launch_bounds__(W_NT, 1) void seq_attention_wide_kernel(const uint1
         for (int x = 0; x < RT; x++) {
             float most = __builtin_fmaxf(top[x], __shfl_xor(top[x], 16));
             most = c * __builtin_fmaxf(most, __shfl_xor(most, 32));
-            const float e_new = most > e_ref[x] + SLACK ? ceilf(most) : e_ref[x];
+            const float e_new = most > e_ref[x] + (SLACK - LIFT) ? ceilf(most) + LIFT : e_ref[x];
             const float f = __builtin_amdgcn_exp2f(e_ref[x] - e_new);
             e_ref[x] = e_new;
 #pragma unroll
@@ -751,13 +759,13 @@ __global__ __launch_bounds__(W_NT, 1) void seq_attention_wide_kernel(const uint1
         for (int x = 0; x < RT; x++) {
             float most = __builtin_fmaxf(top[x], __shfl_xor(top[x], 16));
             most = c * __builtin_fmaxf(most, __shfl_xor(most, 32));
-            if (most > e_ref[x] + SLACK) e_ref[x] = ceilf(most);
+            if (most > e_ref[x] + (SLACK - LIFT)) e_ref[x] = ceilf(most) + LIFT;
         }
     };
     auto some_exceed = [&]() __attribute__((always_inline)) {
         bool up = false;
 #pragma unroll
-        for (int x = 0; x < RT; x++) up |= c * top[x] > e_ref[x] + SLACK;
+        for (int x = 0; x < RT; x++) up |= c * top[x] > e_ref[x] + (SLACK - LIFT);
         return __builtin_amdgcn_ballot_w64(up) != 0;
     };
     // element t (of 8 RT) of a step's exponentials
