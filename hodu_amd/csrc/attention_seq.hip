@@ -232,6 +232,10 @@ template <int D, bool F8> struct R16Geom : SeqGeom<D, F8> {
 template <int CK> struct Slack {
     static constexpr float SLACK = 12.f, LIFT = CK == mfma::CK_F16 ? 0.f : SLACK;
 };
+// The reference of a row without a key yet.  (Finite, so that a score that is masked, -infinity, is 2^-infinity = 0 of it.)
+constexpr float NO_KEY = -__FLT_MAX__;
+// c = scale log2 e, kept normal: a masked score times c stays -infinity
+__device__ __forceinline__ float exponent_scale(float c) { return c < __FLT_MIN__ ? __FLT_MIN__ : c; }
 // 1.0 in every element: the row sums are one more tile of the second product, over the P that it multiplies (which is rounded,
 // so that the weights sum to one), and cost no vector instruction and no exchange between a row's lanes
 template <int CK> __device__ __forceinline__ u32x4_t ones() {
@@ -274,7 +278,7 @@ __global__ __launch_bounds__(R16_NT) void seq_attention_r16_kernel(const uint16_
 #pragma unroll
     for (int ks = 0; ks < G::KS; ks++)
         qf[ks] = *reinterpret_cast<const u32x4_t *>(Q + (q0 + tok) * a.q_token + head * a.q_head + 32 * ks + 8 * g);
-    const float c = a.scale_log2e * (F8 ? a.k_scale[kvh] : 1.f);
+    const float c = exponent_scale(a.scale_log2e * (F8 ? a.k_scale[kvh] : 1.f));
     const float v_scale = F8 ? a.v_scale[kvh] : 1.f;
 
     char *ring = smem + wave * G::WAVE;
@@ -327,9 +331,10 @@ __global__ __launch_bounds__(R16_NT) void seq_attention_r16_kernel(const uint16_
     int v_lane[G::VB];
 #pragma unroll
     for (int b = 0; b < G::VB; b++) v_lane[b] = G::v_lane(r, g, b);
-    // the exponent reference, an integer that moves only when a score exceeds it by 2^SLACK: see the wide kernel below
+    // The reference of the lane's row is a score, the largest when it was last moved; p = 2^(c (s - reference) - LIFT).  The difference is
+    // taken of the scores themselves, where it is exact if they are close, however large they are.
     constexpr float SLACK = Slack<CK>::SLACK, LIFT = Slack<CK>::LIFT;
-    float e_ref = -1e30f;
+    float ref = NO_KEY;
     if (blk0 < blk1) {
         if constexpr (PAGED) fill_window(quot(blk0 * R16_BK, a.page));
         // (pinned: these loads have returned before the ones are issued that the compiler does not know of)
@@ -374,12 +379,12 @@ __global__ __launch_bounds__(R16_NT) void seq_attention_r16_kernel(const uint16_
         float top = sv[0];
 #pragma unroll
         for (int e = 1; e < 8; e++) top = __builtin_fmaxf(top, sv[e]);
-        if (__builtin_amdgcn_ballot_w64(c * top > e_ref + (SLACK - LIFT)) != 0) {
+        if (__builtin_amdgcn_ballot_w64(c * (top - ref) > SLACK) != 0) {
             top = __builtin_fmaxf(top, __shfl_xor(top, 16));
-            top = c * __builtin_fmaxf(top, __shfl_xor(top, 32));
-            const float e_new = top > e_ref + (SLACK - LIFT) ? ceilf(top) + LIFT : e_ref;
-            const float keep = __builtin_amdgcn_exp2f(e_ref - e_new);
-            e_ref = e_new;
+            top = __builtin_fmaxf(top, __shfl_xor(top, 32));
+            const float next = c * (top - ref) > SLACK ? top : ref;
+            const float keep = __builtin_amdgcn_exp2f(c * (ref - next));
+            ref = next;
 #pragma unroll
             for (int j = 0; j <= G::DT; j++)
 #pragma unroll
@@ -387,7 +392,7 @@ __global__ __launch_bounds__(R16_NT) void seq_attention_r16_kernel(const uint16_
         }
         float p[8];
 #pragma unroll
-        for (int e = 0; e < 8; e++) p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[e], c, -e_ref));
+        for (int e = 0; e < 8; e++) p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[e] - ref, c, -LIFT));
         const u32x4_t pf = {pack2<CK>(p[0], p[1]), pack2<CK>(p[2], p[3]), pack2<CK>(p[4], p[5]), pack2<CK>(p[6], p[7])};
         // What P's rounding left is multiplied too, as a second operand: a single token's output is then as exact as its own rounding (the
         // matrix instructions are not the bound here; with P rounded once the error was 1.4 times that).
@@ -428,7 +433,7 @@ __global__ __launch_bounds__(R16_NT) void seq_attention_r16_kernel(const uint16_
     {
         float *mine = mg + (wave * R16 + r) * G::LINE;
         if (g == 0) {
-            mine[0] = e_ref;
+            mine[0] = ref;
             mine[1] = o[G::DT][0];
         }
 #pragma unroll
@@ -437,15 +442,15 @@ __global__ __launch_bounds__(R16_NT) void seq_attention_r16_kernel(const uint16_
     __syncthreads();
     constexpr int PARTS = R16_NT / R16, PER = D / PARTS;  // threads of a row, elements of each
     const int row = tid / PARTS, part = tid % PARTS;
-    float e_all = -1e30f, l = 0.f, x[PER];
+    float all = NO_KEY, l = 0.f, x[PER];
 #pragma unroll
-    for (int i = 0; i < R16_WAVES; i++) e_all = __builtin_fmaxf(e_all, mg[(i * R16 + row) * G::LINE]);
+    for (int i = 0; i < R16_WAVES; i++) all = __builtin_fmaxf(all, mg[(i * R16 + row) * G::LINE]);
 #pragma unroll
     for (int e = 0; e < PER; e++) x[e] = 0.f;
 #pragma unroll
     for (int i = 0; i < R16_WAVES; i++) {
         const float *line = mg + (i * R16 + row) * G::LINE;
-        const float w = __builtin_amdgcn_exp2f(line[0] - e_all);
+        const float w = __builtin_amdgcn_exp2f(c * (line[0] - all));
         l += line[1] * w;
 #pragma unroll
         for (int e = 0; e < PER; e++) x[e] += line[4 + part * PER + e] * w;
@@ -453,19 +458,19 @@ __global__ __launch_bounds__(R16_NT) void seq_attention_r16_kernel(const uint16_
     if (splits > 1) {
         const __amdgpu_buffer_rsrc_t buf = agent_buffer(ws, ws_bytes);
         const unsigned tile_at = blockIdx.x * gridDim.y * R16 * G::LINE * 4, mine = tile_at + (split * R16 + row) * G::LINE * 4;
-        if (part == 0) store16_agent(buf, mine, f32x4_t{e_all, l, 0.f, 0.f});
+        if (part == 0) store16_agent(buf, mine, f32x4_t{all, l, 0.f, 0.f});
 #pragma unroll
         for (int e = 0; e < PER; e += 4) store16_agent(buf, mine + (4 + part * PER + e) * 4, f32x4_t{x[e], x[e + 1], x[e + 2], x[e + 3]});
         int *flag = reinterpret_cast<int *>(smem + G::WINDOW_AT + R16_WAVES * R16_WINDOW * 4);
         if (!arrive_and_check_last(arrival + blockIdx.x, splits, flag, tid)) return;
         // (eight ranges' loads in flight at once: each is a trip to memory)
-        e_all = -1e30f;
+        all = NO_KEY;
         l = 0.f;
 #pragma unroll
         for (int e = 0; e < PER; e++) x[e] = 0.f;
         for (int i0 = 0; i0 < splits; i0 += 8) {
             f32x4_t h[8], y[8][PER / 4];
-            float top = e_all;
+            float top = all;
 #pragma unroll
             for (int u = 0; u < 8; u++) {
                 const unsigned at = tile_at + ((i0 + u < splits ? i0 + u : splits - 1) * R16 + row) * G::LINE * 4;
@@ -475,15 +480,15 @@ __global__ __launch_bounds__(R16_NT) void seq_attention_r16_kernel(const uint16_
             }
 #pragma unroll
             for (int u = 0; u < 8; u++) top = __builtin_fmaxf(top, h[u].x);
-            const float f = __builtin_amdgcn_exp2f(e_all - top);
-            e_all = top;
+            const float f = __builtin_amdgcn_exp2f(c * (all - top));
+            all = top;
             l *= f;
 #pragma unroll
             for (int e = 0; e < PER; e++) x[e] *= f;
 #pragma unroll
             for (int u = 0; u < 8; u++) {
                 if (i0 + u >= splits) break;
-                const float w = __builtin_amdgcn_exp2f(h[u].x - e_all);
+                const float w = __builtin_amdgcn_exp2f(c * (h[u].x - all));
                 l += h[u].y * w;
 #pragma unroll
                 for (int e = 0; e < PER; e++) x[e] += y[u][e / 4][e % 4] * w;
@@ -522,6 +527,10 @@ __global__ __launch_bounds__(R16_NT) void seq_attention_r16_kernel(const uint16_
 // The exponent reference of a row is an integer E, ceil(c max) + LIFT when it was last set, c = scale log2 e; p = 2^(c s - E).  It moves only
 // when a score reaches c s > E + SLACK - LIFT, which the lanes find out without talking to each other (any lane's own maximum); then the
 // row's lanes agree on the new one and O, the row sum and the P not yet multiplied are rescaled -- by a power of two, exactly.
+// That takes |c s| far below 2^24, where E and c s are told apart to less than one.  A wavefront that meets larger ones (its first
+// scores, or one that moves a reference) turns careful: its references become scores, p = 2^(c (s - reference) - LIFT) as in
+// the kernel above, where a difference is exact if the scores are close, and it takes the slow step from there on.  In the
+// loops that would be an instruction per exponential between matrix instructions that are 16 cycles long already.
 // Row tiles per wavefront: 3 at head dim 128 (O, q, two steps' scores and P are 84 registers a tile; with 4 the allocator runs out),
 // 4 at 64.
 template <int D> constexpr int W_TILES = D == 128 ? 3 : 4;
@@ -577,7 +586,7 @@ __global__ __launch_bounds__(W_NT, 1) void seq_attention_wide_kernel(const uint1
 #pragma unroll
         for (int ks = 0; ks < KS; ks++) qf[x][ks] = *reinterpret_cast<const u32x4_t *>(q + 32 * ks + 8 * g);
     }
-    const float c = a.scale_log2e * (F8 ? a.k_scale[kvh] : 1.f);
+    const float c = exponent_scale(a.scale_log2e * (F8 ? a.k_scale[kvh] : 1.f));
     auto last_row = [&](int i) { return i < rows ? i : rows - 1; };
     const int keys_any = a.causal ? quot(last_row(row0 + BM - 1), a.by_group) + m - n + 1 : m;  // keys the tile needs
     int keys = keys_any > 0 ? keys_any : 0;
@@ -609,7 +618,9 @@ __global__ __launch_bounds__(W_NT, 1) void seq_attention_wide_kernel(const uint1
     int window0 = 0;  // first table column in the window
     [[maybe_unused]] auto fill_window = [&](int col0) __attribute__((always_inline)) {
         const int cols = quot(from + keys - 1, a.page) + 1;
-        for (int i = tid; i < W_WINDOW && col0 + i < cols; i += W_NT) {
+        int i = tid;
+        mfma::pin_vector(i);  // (or the compiler keeps addresses made from it in registers throughout the kernel)
+        for (; i < W_WINDOW && col0 + i < cols; i += W_NT) {
             const int pg = a.table[(long)b * a.width + col0 + i];
             window[i] = pg < 0 ? 0 : pg < a.n_pages ? pg : a.n_pages - 1;
         }
@@ -676,7 +687,7 @@ __global__ __launch_bounds__(W_NT, 1) void seq_attention_wide_kernel(const uint1
     for (int x = 0; x < RT; x++) {
 #pragma unroll
         for (int j = 0; j <= DT; j++) o[x][j] = acc_t{0.f, 0.f, 0.f, 0.f};
-        e_ref[x] = -1e30f;  // no key yet
+        e_ref[x] = NO_KEY;
     }
 
     constexpr int KF = G::KF, VR = G::VR;
@@ -728,39 +739,72 @@ __global__ __launch_bounds__(W_NT, 1) void seq_attention_wide_kernel(const uint1
             for (int e = 1; e < 8; e++) top[x] = __builtin_fmaxf(top[x], sc[x][e >> 2][e & 3]);
         }
     };
+    constexpr float SLACK = Slack<CK>::SLACK, LIFT = Slack<CK>::LIFT;
+    int careful = 0;  // 1: the wavefront's references are scores (see above)
+    constexpr float MOST = 0x1p22f;
+    // the row's largest new score, the same in its four lanes
+    auto row_top = [&](int x) __attribute__((always_inline)) {
+        const float most = __builtin_fmaxf(top[x], __shfl_xor(top[x], 16));
+        return __builtin_fmaxf(most, __shfl_xor(most, 32));
+    };
     // Moves the references of the rows whose new scores exceed them by too much (rare: some lane saw one); pc: the P that is
     // still to be multiplied
-    constexpr float SLACK = Slack<CK>::SLACK, LIFT = Slack<CK>::LIFT;
     auto move_references = [&](u32x4_t (&pc)[RT]) __attribute__((always_inline)) {
         mfma::mfma_results_settle();
         __builtin_amdgcn_sched_barrier(0);
+        float most[RT], f[RT];
+        bool far = false;
 #pragma unroll
         for (int x = 0; x < RT; x++) {
-            float most = __builtin_fmaxf(top[x], __shfl_xor(top[x], 16));
-            most = c * __builtin_fmaxf(most, __shfl_xor(most, 32));
-            const float e_new = most > e_ref[x] + (SLACK - LIFT) ? ceilf(most) + LIFT : e_ref[x];
-            const float f = __builtin_amdgcn_exp2f(e_ref[x] - e_new);
-            e_ref[x] = e_new;
+            most[x] = row_top(x);
+            f[x] = 1.f;
+            far |= !(c * most[x] <= MOST) && most[x] > 0.f;  // (only a score that is larger than the reference moves it)
+        }
+        if (!careful && __builtin_amdgcn_ballot_w64(far) != 0) {
+            careful = 1;
 #pragma unroll
-            for (int j = 0; j <= DT; j++) mfma::scale4_acc(o[x][j], f);
+            for (int x = 0; x < RT; x++)
+                if (e_ref[x] != NO_KEY) {
+                    const float e = e_ref[x] - LIFT, s = e / c, ref = __builtin_fminf(s, __FLT_MAX__);
+                    f[x] = __builtin_amdgcn_exp2f(__builtin_fmaf(-ref, c, e));
+                    e_ref[x] = ref;
+                }
+        }
+#pragma unroll
+        for (int x = 0; x < RT; x++) {
+            const float from = e_ref[x];
+            if (careful) {
+                if (c * (most[x] - from) > SLACK) e_ref[x] = most[x];
+                f[x] *= __builtin_amdgcn_exp2f(c * (from - e_ref[x]));
+            } else {
+                if (c * most[x] > from + (SLACK - LIFT)) e_ref[x] = ceilf(c * most[x]) + LIFT;
+                f[x] = __builtin_amdgcn_exp2f(from - e_ref[x]);
+            }
+#pragma unroll
+            for (int j = 0; j <= DT; j++) mfma::scale4_acc(o[x][j], f[x]);
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 const uint32_t pw = pc[x][i];
-                if constexpr (!F16) pc[x][i] = pack2<CK>(bf16_bits_to_f32((uint16_t)pw) * f, bf16_bits_to_f32((uint16_t)(pw >> 16)) * f);
-                else pc[x][i] = pack2<CK>(f16_bits_to_f32((uint16_t)pw) * f, f16_bits_to_f32((uint16_t)(pw >> 16)) * f);
+                if constexpr (!F16) pc[x][i] = pack2<CK>(bf16_bits_to_f32((uint16_t)pw) * f[x], bf16_bits_to_f32((uint16_t)(pw >> 16)) * f[x]);
+                else pc[x][i] = pack2<CK>(f16_bits_to_f32((uint16_t)pw) * f[x], f16_bits_to_f32((uint16_t)(pw >> 16)) * f[x]);
             }
         }
         mfma::mfma_results_settle();
         __builtin_amdgcn_sched_barrier(0);
     };
-    // the first ones: there is nothing to rescale yet
+    // the first ones: there is nothing to rescale yet.  (The keys that a row attends begin with the first one: a row without a key here has none.)
     auto set_references = [&]() __attribute__((always_inline)) {
+        float most[RT];
+        bool far = false;
 #pragma unroll
         for (int x = 0; x < RT; x++) {
-            float most = __builtin_fmaxf(top[x], __shfl_xor(top[x], 16));
-            most = c * __builtin_fmaxf(most, __shfl_xor(most, 32));
-            if (most > e_ref[x] + (SLACK - LIFT)) e_ref[x] = ceilf(most) + LIFT;
+            most[x] = row_top(x);
+            far |= most[x] > -INFINITY && !(__builtin_fabsf(c * most[x]) <= MOST);
         }
+        careful = __builtin_amdgcn_ballot_w64(far) != 0 ? 1 : 0;
+#pragma unroll
+        for (int x = 0; x < RT; x++)
+            if (most[x] > -INFINITY) e_ref[x] = careful ? most[x] : ceilf(c * most[x]) + LIFT;
     };
     auto some_exceed = [&]() __attribute__((always_inline)) {
         bool up = false;
@@ -768,11 +812,22 @@ __global__ __launch_bounds__(W_NT, 1) void seq_attention_wide_kernel(const uint1
         for (int x = 0; x < RT; x++) up |= c * top[x] > e_ref[x] + (SLACK - LIFT);
         return __builtin_amdgcn_ballot_w64(up) != 0;
     };
+    auto some_exceed_scores = [&]() __attribute__((always_inline)) {
+        bool up = false;
+#pragma unroll
+        for (int x = 0; x < RT; x++) up |= c * (top[x] - e_ref[x]) > SLACK;
+        return __builtin_amdgcn_ballot_w64(up) != 0;
+    };
     // element t (of 8 RT) of a step's exponentials
     float pair;
-    auto exponential = [&](const acc_t (&sc)[RT][2], u32x4_t (&pc)[RT], int t) __attribute__((always_inline)) {
+    auto exponential = [&](auto either, const acc_t (&sc)[RT][2], u32x4_t (&pc)[RT], int t) __attribute__((always_inline)) {
         const int x = t >> 3, e = t & 7;
-        const float v = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[x][e >> 2][e & 3], c, -e_ref[x]));
+        float s = sc[x][e >> 2][e & 3], less = e_ref[x];
+        if constexpr (decltype(either)::value) {
+            s -= careful ? less : 0.f;
+            less = careful ? LIFT : less;
+        }
+        const float v = __builtin_amdgcn_exp2f(__builtin_fmaf(s, c, -less));
         if (e & 1) {
             pc[x][e >> 1] = pack2<CK>(pair, v);
             uint32_t w = pc[x][e >> 1];
@@ -813,7 +868,7 @@ __global__ __launch_bounds__(W_NT, 1) void seq_attention_wide_kernel(const uint1
                 Cmp::mma(v_operand(u / RT), pp[u % RT], o[u % RT][u / RT]);
                 if (u >= NP - RT) Cmp::mma(one, pp[u % RT], o[u % RT][DT]);
             }
-            if (t % EVERY == 0) exponential(sc, pc, t / EVERY);
+            if (t % EVERY == 0) exponential(std::false_type(), sc, pc, t / EVERY);
             const int soon = t + AHEAD;  // the instruction whose fragment is read now, if it is the first to use it
             if (soon < NQ) {
                 if (soon % RT == 0) read_k(soon / RT, k_block);
@@ -867,7 +922,7 @@ __global__ __launch_bounds__(W_NT, 1) void seq_attention_wide_kernel(const uint1
         if (i > 0) times_v(i - 1, pc);
         if (i >= 0)
 #pragma unroll
-            for (int t = 0; t < EL; t++) exponential(sc, pc, t);
+            for (int t = 0; t < EL; t++) exponential(std::true_type(), sc, pc, t);
         const int at = k_of(i + 1);
 #pragma unroll
         for (int q = 0; q < KF; q++) read_k(q, at);
@@ -940,7 +995,8 @@ __global__ __launch_bounds__(W_NT, 1) void seq_attention_wide_kernel(const uint1
         set_references();
         int i = 0;  // the step in front of us; i = 2 st + 1: in the middle of a stage
         while (st < stages) {
-            if (!(i & 1) && i <= steps) {
+            mfma::pin_scalar(careful);  // (or the compiler makes a loop of its own for either value, and spills in them)
+            if (!careful && !(i & 1) && i <= steps) {
                 acc_t sn[RT][2];     // scores of the odd steps, those of the even ones in sc
                 u32x4_t pn[RT];      // P of the even steps, that of the odd ones in pc
                 first_fragments(k_of(2 * st + 1));
@@ -981,7 +1037,7 @@ __global__ __launch_bounds__(W_NT, 1) void seq_attention_wide_kernel(const uint1
                 i++;
                 if (!(i & 1)) st++;
             }
-            if (i <= steps && some_exceed()) move_references(pc);
+            if (i <= steps && (careful ? some_exceed_scores() : some_exceed())) move_references(pc);
         }
         if (steps == 2 * stages) times_v(steps - 1, pc);  // P V of the last step
     }
@@ -996,7 +1052,7 @@ __global__ __launch_bounds__(W_NT, 1) void seq_attention_wide_kernel(const uint1
             if (wrow0 < rows) {
 #pragma unroll
                 for (int x = 0; x < RT; x++) {
-                    store16_agent(buf, mine + x * (DT + 1) * 1024, f32x4_t{e_ref[x], o[x][DT][0], 0.f, 0.f});
+                    store16_agent(buf, mine + x * (DT + 1) * 1024, f32x4_t{careful ? e_ref[x] : 0.f, careful ? LIFT : e_ref[x], o[x][DT][0], 0.f});
 #pragma unroll
                     for (int j = 0; j < DT; j++)
                         store16_agent(buf, mine + (x * (DT + 1) + 1 + j) * 1024, f32x4_t{o[x][j][0], o[x][j][1], o[x][j][2], o[x][j][3]});
@@ -1007,14 +1063,14 @@ __global__ __launch_bounds__(W_NT, 1) void seq_attention_wide_kernel(const uint1
 #pragma unroll
                 for (int x = 0; x < RT; x++) {
                     const unsigned row_at = tile_at + x * (DT + 1) * 1024;
-                    float e_all = -1e30f, l = 0.f;
+                    // a range's p are 2^(c (s - score) - e): in the common scale its weight is 2^(c score + e)
+                    float score = 0.f, e = 0.f, l = 0.f;
                     f32x4_t y[DT];
 #pragma unroll
                     for (int j = 0; j < DT; j++) y[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
                     // (four ranges' loads in flight at once)
                     for (int i0 = 0; i0 < splits; i0 += 4) {
                         f32x4_t h[4], part[4][DT];
-                        float most = e_all;
 #pragma unroll
                         for (int u = 0; u < 4; u++) {
                             const unsigned at = row_at + (i0 + u < splits ? i0 + u : splits - 1) * SLICE;
@@ -1023,23 +1079,20 @@ __global__ __launch_bounds__(W_NT, 1) void seq_attention_wide_kernel(const uint1
                             for (int j = 0; j < DT; j++) part[u][j] = load16_agent<f32x4_t>(buf, at + (1 + j) * 1024);
                         }
 #pragma unroll
-                        for (int u = 0; u < 4; u++) most = __builtin_fmaxf(most, h[u].x);
-                        const float f = __builtin_amdgcn_exp2f(e_all - most);
-                        e_all = most;
-                        l *= f;
-#pragma unroll
-                        for (int j = 0; j < DT; j++)
-#pragma unroll
-                            for (int e = 0; e < 4; e++) y[j][e] *= f;
-#pragma unroll
                         for (int u = 0; u < 4; u++) {
                             if (i0 + u >= splits) break;
-                            const float w = __builtin_amdgcn_exp2f(h[u].x - e_all);
-                            l += h[u].y * w;
+                            // the larger of the two stays as it is; one without a key, whose sum is zero, has no say in the scale
+                            const float more = __builtin_fmaf(h[u].x - score, c, h[u].y - e);
+                            const bool none = h[u].z == 0.f, takes = !none && (l == 0.f || more > 0.f);
+                            const float keep = takes ? l == 0.f ? 0.f : __builtin_amdgcn_exp2f(-more) : 1.f;
+                            const float w = none ? 0.f : takes ? 1.f : __builtin_amdgcn_exp2f(more);
+                            score = takes ? h[u].x : score;
+                            e = takes ? h[u].y : e;
+                            l = l * keep + h[u].z * w;
 #pragma unroll
                             for (int j = 0; j < DT; j++)
 #pragma unroll
-                                for (int e = 0; e < 4; e++) y[j][e] += part[u][j][e] * w;
+                                for (int n2 = 0; n2 < 4; n2++) y[j][n2] = y[j][n2] * keep + part[u][j][n2] * w;
                         }
                     }
                     o[x][DT][0] = l;

@@ -57,6 +57,10 @@ __device__ __forceinline__ void scale4_acc(f32x4_acc_t &c, float s) {
 // an empty statement that takes and returns a value: it is there by then, and in this register file
 template <class T> __device__ __forceinline__ void pin_vector(T &v) { asm volatile("" : "+v"(v)); }
 template <class T> __device__ __forceinline__ void pin_accumulation(T &v) { asm volatile("" : "+a"(v)); }
+__device__ __forceinline__ void pin_scalar(int &v) {
+    v = __builtin_amdgcn_readfirstlane(v);
+    asm volatile("" : "+s"(v));
+}
 
 // v_mfma_scale_f32_16x16x128_f8f6f4 with unit scales (scale bytes 0x7F = 2^0), both operands of one 8-bit float format
 // (FMT 0 = e4m3, 1 = e5m2: the instruction's cbsz / blgp fields), the accumulator tied as above -- left to the register

@@ -328,7 +328,9 @@ int hodu_rocm_paged_store(hodu_rocm_ctx *ctx, int dtype, int cache_dtype, const 
  * h / (heads / kv_heads).  causal != 0: row i of n rows over m keys attends keys 0 .. i + m - n (the last row all of
  * them).  A row that attends no key is zero; rows of out behind the last sequence are left as they were; offsets are
  * clamped to the packed lengths.  Scores, softmax and the sums over keys are f32; the probabilities are rounded to
- * `dtype` as the second product's operand and the result once.  out: contiguous [q_tokens, heads, D].  A key that a row
+ * `dtype` as the second product's operand and the result once.  Scores that f32 holds may be as large and as far apart as
+ * they like (some of 2^22 / scale and beyond in prompts and chunks are worked on slowly), and values as large as keeps the sum of
+ * their sizes over the keys within f32.  out: contiguous [q_tokens, heads, D].  A key that a row
  * does not attend has no part in the row, whatever it is; a VALUE of the row's own sequence that is not finite may make
  * the row NaN although the row does not attend it (zero times infinity), values of other sequences never do.
  * dtype: bf16 or f16; D = 64 or 128; the D elements dense, strides and offsets multiples of 8 elements, bases of 16

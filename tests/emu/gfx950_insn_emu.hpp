@@ -342,6 +342,7 @@ template <bool F16, bool NOPS = false> inline void mfma16_first(const emu_u32x4 
 }
 template <class T> inline void pin_vector(T &) {}
 template <class T> inline void pin_accumulation(T &) {}
+inline void pin_scalar(int &) {}
 inline void scale4_acc(f32x4_acc_t &c, float s) { for (int e = 0; e < 4; e++) c[e] *= s; }
 inline void mfma_results_settle() {}
 

@@ -19,7 +19,7 @@ def ctx():
     c.close()
 
 
-def varlen(ctx, tile, dt, q, k, v, causal):
+def varlen(ctx, tile, dt, q, k, v, causal, scale=None):
     """(bits, values) of one sequence's outputs; q [n, Hq, D], k and v [m, Hk, D] float64, values of dt"""
     n, hq, d = q.shape
     m, hk, _ = k.shape
@@ -30,7 +30,8 @@ def varlen(ctx, tile, dt, q, k, v, causal):
     qo, ko = ctx.upload(np.array([0, n], np.int32)), ctx.upload(np.array([0, m], np.int32))
     ctx.force_tile(tile)
     try:
-        ctx.attention_varlen(dt, *operands, out, qo, ko, ffi.varlen_md(1, n, m, hq, hk, d), S.scalar(d, dt)[0], causal)
+        ctx.attention_varlen(dt, *operands, out, qo, ko, ffi.varlen_md(1, n, m, hq, hk, d),
+                             S.scalar(d, dt)[0] if scale is None else S.to_bits(np.array([scale]), dt), causal)
     finally:
         ctx.force_tile(-1)
     bits = ctx.download(out, np.uint16).reshape(n, hq, d)
@@ -105,3 +106,96 @@ def test_scores_that_rise_step_by_step(ctx, tile, dt):
         for causal in (True, False):
             _, got = varlen(ctx, tile, dt, q, k, v, causal)
             check(got, q, k, v, dt, causal, f"steps of {step}", d)
+
+
+def check_exact_scores(got, q, k, v, dt, causal, what, scale=None):
+    """For scores that are exact in f32 (one product, or a power of two and a small whole number), where what they are does not enter the
+    bound, only what they differ by.  With u half a step of dt and e = 2^-24: P is rounded to dt, and once more where
+    a reference moves before it is multiplied: 2 u a (a = sum of p |v|); a P whose exponent is below -64 is nothing,
+    the argument of the others is off by three roundings of up to 64 e each, the exponential by 8 e, the same again in the
+    row sum; sums over m keys (m + 8) e a; the rounded row sum and the result u |o| each; an f16 P below its normal
+    range, and an f16 result, by 2^-25 as in seq_util.allowed."""
+    n, hq, d = q.shape
+    scale = S.scalar(d, dt)[1] if scale is None else scale
+    o, a, _, inv = S.attend(q, k, v, scale, causal)
+    u, e, m = S.HALF_STEP[dt], 2.0 ** -24, k.shape[0]
+    tol = a * (2 * u + 2 * (8 * e + 3 * 64 * e) + (m + 8) * e) + 2 * np.abs(o) * u
+    if dt == "f16":
+        tol = tol + (m * 2.0 ** -25 * inv * np.abs(v).max())[..., None] + 2.0 ** -25
+    off = np.abs(got - o)
+    bad = ~(off <= tol * (1 + 2 * u))
+    assert not bad.any(), f"{what}: {bad.sum()} of {bad.size} wrong, first at {np.argwhere(bad)[0].tolist()}: got {got[tuple(np.argwhere(bad)[0])]}, " \
+                          f"want {o[tuple(np.argwhere(bad)[0])]}"
+
+
+def one_product(m, n, d, dt, q0, scores, seed):
+    """q and k whose product is q0 * scores, one element of the head dim each (key by key; the same for all rows but every third,
+    which is zero: an ordinary row among them), and values"""
+    g = np.random.default_rng(seed)
+    q, k = np.zeros((n, 1, d)), np.zeros((m, 1, d))
+    q[:, 0, 5] = q0
+    q[2::3] = 0
+    k[:, 0, 5] = scores
+    return q, rounded(k, dt), rounded(g.standard_normal((m, 1, d)), dt)
+
+
+@pytest.mark.parametrize("tile", TILES)
+@pytest.mark.parametrize("dt,d", [("bf16", 64), ("f16", 128)])
+def test_scores_larger_than_their_differences_can_be(ctx, tile, dt, d):
+    """scores so large that a step of f32 between them is a factor of more than 2^100: equal ones share the row, the larger one of two takes it"""
+    n, m = 7, 150
+    big, unit = (1e30, 1.0) if dt == "bf16" else (4.9e4, 5e4)
+    for name, scores in (("equal", np.full(m, big)), ("equal, negative", np.full(m, -big)), ("all but the first", np.r_[0, np.full(m - 1, -big)]),
+                         ("one in the middle", np.r_[np.full(m // 2, -big), big, np.full(m - m // 2 - 1, -big)]),
+                         ("the last ones", np.r_[np.full(m - 3, big / 2), np.full(3, big)]), ("from negative to zero", np.r_[np.full(100, -big), np.zeros(m - 100)]),
+                         ("falling", -big * np.arange(1, m + 1) / m), ("rising", big * np.arange(1, m + 1) / m), ("in pairs", big * (np.arange(m) // 2) / m),
+                         ("ordinary, then large", np.r_[np.linspace(-1, 1, 70) / unit, np.full(m - 70, big)])):
+        q, k, v = one_product(m, n, d, dt, unit, scores, len(name))
+        q = rounded(q, dt)
+        for causal in (False, True):
+            _, got = varlen(ctx, tile, dt, q, k, v, causal)
+            check_exact_scores(got, q, k, v, dt, causal, f"{name}, causal {causal}")
+        _, got = paged(ctx, tile, dt, q, k, v, cut=400)
+        check_exact_scores(got, q, k, v, dt, True, f"{name}, cached")
+
+
+@pytest.mark.parametrize("tile", TILES)
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+def test_small_differences_of_large_scores(ctx, tile, dt):
+    """scores of 2^24 to 2^28 that differ by a few steps of f32: exact, and so are their differences"""
+    d, n, m = 64, 4, 200
+    for size, step in ((13, 8.0), (14, 32.0), (12, 2.0), (-13, 8.0)):
+        g = np.random.default_rng(abs(size))
+        q, k = np.zeros((n, 1, d)), np.zeros((m, 1, d))
+        q[:, 0, 0], q[:, 0, 1] = 2.0 ** abs(size), 1
+        k[:, 0, 0] = np.sign(size) * 2.0 ** abs(size)
+        k[:, 0, 1] = step * g.integers(0, 12, m)
+        v = rounded(g.standard_normal((m, 1, d)), dt)
+        for causal in (False, True):
+            _, got = varlen(ctx, tile, dt, q, k, v, causal)
+            check_exact_scores(got, q, k, v, dt, causal, f"2^{2 * abs(size)}")
+        _, got = paged(ctx, tile, dt, q, k, v, cut=400)
+        check_exact_scores(got, q, k, v, dt, True, f"2^{2 * abs(size)}, cached")
+
+
+@pytest.mark.parametrize("tile", TILES)
+def test_scores_beyond_f32_once_they_are_scaled(ctx, tile):
+    for q0, scores, scale in ((1.0, np.full(90, -2.0 ** 127), 8.0), (1.0, np.r_[np.full(60, -2.0 ** 127), np.full(30, -2.0 ** 126)], 4.0), (1.0, np.full(90, 2.0 ** 127), 8.0),
+                              (2.0 ** -100, np.full(90, 2.0 ** 10), 2.0 ** -130)):
+        q, k, v = one_product(90, 7, 64, "bf16", q0, scores, 3)
+        _, got = varlen(ctx, tile, "bf16", q, k, v, True, scale)
+        check_exact_scores(got, q, k, v, "bf16", True, f"{scores[0]} scaled by {scale}", scale)
+
+
+@pytest.mark.parametrize("tile", TILES)
+def test_ranges_of_keys_with_scores_far_apart_are_added(ctx, tile):
+    """keys cut across workgroups: each range's reference is of its own size"""
+    for dt, big in (("bf16", 1e30), ("f16", 6e4)):
+        m, d = 1500, 64
+        for name, scores in (("the first range", np.r_[np.full(300, big), np.zeros(m - 300)]), ("the last range", np.r_[np.zeros(m - 10), np.full(10, big)]),
+                             ("negative but for the middle", np.r_[np.full(700, -big), np.linspace(-1, 1, 100) / big, np.full(m - 800, -big)]),
+                             ("all negative", np.full(m, -big)), ("rising", big * (np.arange(m) // 4) / m)):
+            q, k, v = one_product(m, 9, d, dt, 1.0 if dt == "bf16" else 6e4, scores, 4)
+            q = rounded(q, dt)
+            _, got = paged(ctx, tile, dt, q, k, v, cut=100)
+            check_exact_scores(got, q, k, v, dt, True, f"{dt}: {name}")
