@@ -324,8 +324,14 @@ __global__ __launch_bounds__(R16_NT) void seq_attention_r16_kernel(const uint16_
     };
 
     acc_t o[G::DT + 1];  // the last tile: the row sums
+    // What the remainders of P give is summed apart from what P gives: of an infinite value P makes an infinity, a remainder may make its
+    // opposite or, where it is zero, a NaN.  (8-bit values have no infinity.)
+    constexpr bool APART = !F8;
+    acc_t o_rest[APART ? G::DT : 1];
 #pragma unroll
     for (int j = 0; j <= G::DT; j++) o[j] = acc_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < (APART ? G::DT : 1); j++) o_rest[j] = acc_t{0.f, 0.f, 0.f, 0.f};
     const u32x4_t one = ones<CK>();
     const int k_lane = G::k_lane(r, g);
     int v_lane[G::VB];
@@ -353,7 +359,18 @@ __global__ __launch_bounds__(R16_NT) void seq_attention_r16_kernel(const uint16_
         else if (G::RING > 2 && later == 1) __builtin_amdgcn_s_waitcnt(mfma::waitcnt_vm_lgkm0(2 * G::DMAS));
         else __builtin_amdgcn_s_waitcnt(mfma::waitcnt_vm_lgkm0(0));
         mfma::wave_lds_fence();
-        const char *kl = ring + slot * G::BLOCK, *vl = kl + G::BLOCK_K;
+        char *kl = ring + slot * G::BLOCK, *vl = kl + G::BLOCK_K;
+        if constexpr (APART) {
+            // the copies of the last key, which P is zero of: an infinite value times zero would be a NaN
+            if ((blk + 1) * R16_BK > keys) {
+#pragma unroll
+                for (int i = 0; i < G::DMAS; i++)
+                    if (blk * R16_BK + i * G::KPI + lane / G::CPR >= keys)
+                        *reinterpret_cast<u32x4_t *>(vl + i * G::PADDED_V + lane * 16) = u32x4_t{0, 0, 0, 0};
+                __builtin_amdgcn_s_waitcnt(mfma::waitcnt_vm_lgkm0(63));
+                mfma::wave_lds_fence();
+            }
+        }
 
         acc_t s[2];
 #pragma unroll
@@ -388,7 +405,11 @@ __global__ __launch_bounds__(R16_NT) void seq_attention_r16_kernel(const uint16_
 #pragma unroll
             for (int j = 0; j <= G::DT; j++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) o[j][e] *= keep;
+                for (int e = 0; e < 4; e++) {
+                    o[j][e] *= keep;
+                    if constexpr (APART)
+                        if (j < G::DT) o_rest[j][e] *= keep;
+                }
         }
         float p[8];
 #pragma unroll
@@ -416,7 +437,8 @@ __global__ __launch_bounds__(R16_NT) void seq_attention_r16_kernel(const uint16_
                 vf = u32x4_t{lo.x, lo.y, hi.x, hi.y};
             }
             Cmp::mma(vf, pf, o[j]);
-            Cmp::mma(vf, pr, o[j]);
+            if constexpr (APART) Cmp::mma(vf, pr, o_rest[j]);
+            else Cmp::mma(vf, pr, o[j]);
         }
         if (blk + G::RING < blk1) {
             // the block's reads have been answered before its slot's next loads are issued
@@ -427,6 +449,12 @@ __global__ __launch_bounds__(R16_NT) void seq_attention_r16_kernel(const uint16_
         slot = slot + 1 < G::RING ? slot + 1 : 0;
     }
 
+    if constexpr (APART) {
+#pragma unroll
+        for (int j = 0; j < G::DT; j++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) o[j][e] += __builtin_fabsf(o[j][e]) == INFINITY ? 0.f : o_rest[j][e];
+    }
     // ---- the four wavefronts meet: per wavefront and row (reference, sum, -, -, O) ----
     __syncthreads();
     float *mg = reinterpret_cast<float *>(smem);
@@ -970,6 +998,21 @@ __global__ __launch_bounds__(W_NT, 1) void seq_attention_wide_kernel(const uint1
             // and everybody is done with what this stage's loads overwrite
             if (st > 0 && st + 2 < stages) __builtin_amdgcn_s_waitcnt(mfma::waitcnt_vm_lgkm0(2 * G::NI));
             else __builtin_amdgcn_s_waitcnt(mfma::waitcnt_vm_lgkm0(0));
+            if constexpr (!F8) {
+                // the copies of the last key, which P is zero of: an infinite value times zero would be a NaN.  (Each wavefront its own,
+                // which have landed; 8-bit values have no infinity.)
+                if ((st + 1) * W_BK > keys) {
+                    int l = lane;
+                    mfma::pin_vector(l);  // (no address of this is kept in a register elsewhere)
+#pragma unroll
+                    for (int p = 0; p < G::NI; p++) {
+                        const int at = wave * G::NI + p;
+                        if (st * W_BK + at * G::KPI + l / G::CPR >= keys)
+                            *reinterpret_cast<u32x4_t *>(smem + G::V_AT + (st & (W_RING - 1)) * 2 * G::BLOCK_V + at * G::PADDED_V + l * 16) = u32x4_t{0, 0, 0, 0};
+                    }
+                    __builtin_amdgcn_s_waitcnt(mfma::waitcnt_vm_lgkm0(0));
+                }
+            }
             __syncthreads();
             if (st + 2 < stages) issue(st + 2, true);
             if (st + 3 < stages) issue(st + 3, false);
@@ -1107,9 +1150,12 @@ __global__ __launch_bounds__(W_NT, 1) void seq_attention_wide_kernel(const uint1
     }
 
     // ---- O / l, one rounding: lane (r, g) holds row r of each tile, head-dim columns 16 j + 4 g + e ----
+    int l_end = lane;
+    mfma::pin_vector(l_end);  // (the rows are counted anew: kept from the beginning they take a register that the loops want)
+    const int r_end = l_end & 15, g_end = l_end >> 4;
 #pragma unroll
     for (int x = 0; x < RT; x++) {
-        const int row = wrow0 + 16 * x + r;
+        const int row = wrow0 + 16 * x + r_end;
         const float l = o[x][DT][0];
         const float inv = l == 0.f ? 0.f : (F8 ? a.v_scale[kvh] : 1.f) / l;  // a row without keys is zero
         if (row >= rows) continue;
@@ -1117,7 +1163,7 @@ __global__ __launch_bounds__(W_NT, 1) void seq_attention_wide_kernel(const uint1
         uint16_t *dst = O + ((long)(q0 + tok) * a.heads + head) * D;
 #pragma unroll
         for (int j = 0; j < DT; j++)
-            *reinterpret_cast<u32x2_t *>(dst + 16 * j + 4 * g) =
+            *reinterpret_cast<u32x2_t *>(dst + 16 * j + 4 * g_end) =
                 u32x2_t{pack2<CK>(o[x][j][0] * inv, o[x][j][1] * inv), pack2<CK>(o[x][j][2] * inv, o[x][j][3] * inv)};
     }
 }

@@ -332,7 +332,8 @@ int hodu_rocm_paged_store(hodu_rocm_ctx *ctx, int dtype, int cache_dtype, const 
  * they like (some of 2^22 / scale and beyond in prompts and chunks are worked on slowly), and values as large as keeps the sum of
  * their sizes over the keys within f32.  out: contiguous [q_tokens, heads, D].  A key that a row
  * does not attend has no part in the row, whatever it is; a VALUE of the row's own sequence that is not finite may make
- * the row NaN although the row does not attend it (zero times infinity), values of other sequences never do.
+ * the row NaN although the row does not attend it (zero times infinity), values of other sequences never do.  An infinite
+ * value that a row attends makes its column infinite, unless the key's probability rounds to zero in `dtype` (NaN).
  * dtype: bf16 or f16; D = 64 or 128; the D elements dense, strides and offsets multiples of 8 elements, bases of 16
  * bytes; scale: the scalar in `dtype`, positive and finite.  HODU_ROCM_UNSUPPORTED otherwise.
  * metadata: [batch, q_tokens, k_tokens, heads, kv_heads, D, q_token, q_head, k_token, k_head, v_token, v_head, q_off,

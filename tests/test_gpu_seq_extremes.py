@@ -25,7 +25,7 @@ def varlen(ctx, tile, dt, q, k, v, causal, scale=None):
     m, hk, _ = k.shape
     operands = [ctx.upload(S.to_bits(x, dt)) for x in (q, k, v)]
     for x, buf in zip((q, k, v), operands):
-        assert np.array_equal(S.widen(S.to_bits(x, dt), dt).reshape(x.shape), x)
+        assert np.array_equal(S.widen(S.to_bits(x, dt), dt).reshape(x.shape), x, equal_nan=True)
     out = ctx.alloc(n * hq * d * 2)
     qo, ko = ctx.upload(np.array([0, n], np.int32)), ctx.upload(np.array([0, m], np.int32))
     ctx.force_tile(tile)
@@ -199,3 +199,32 @@ def test_ranges_of_keys_with_scores_far_apart_are_added(ctx, tile):
             q = rounded(q, dt)
             _, got = paged(ctx, tile, dt, q, k, v, cut=100)
             check_exact_scores(got, q, k, v, dt, True, f"{dt}: {name}")
+
+
+@pytest.mark.parametrize("tile", TILES)
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+def test_infinite_values_that_are_attended(ctx, tile, dt):
+    """an infinity among a row's values is the row's result in its column, infinities of both signs or a NaN make it NaN, and the other
+    columns are what they would be"""
+    n, d = 9, 64
+    for m, at in ((40, 0), (300, 0), (300, 37), (300, 299), (1500, 700)):
+        g = np.random.default_rng(m + at)
+        q, k = rounded(g.standard_normal((n, 2, d)), dt), rounded(g.standard_normal((m, 1, d)) * 0.3, dt)
+        k[3::5] = k[2::5][:len(k[3::5])]  # (equal scores among them: probabilities that have no remainder, or the same one)
+        v = rounded(g.standard_normal((m, 1, d)), dt)
+        finite = v.copy()
+        for col, word in ((1, np.inf), (6, -np.inf), (17, np.nan), (40, np.inf), (63, -np.inf)):
+            v[at, 0, col], finite[at, 0, col] = word, 0.0
+        v[(at + 1) % n, 0, 40], finite[(at + 1) % n, 0, 40] = -np.inf, 0.0
+        if at < n:  # every row attends the key
+            calls = [varlen(ctx, tile, dt, q, k, v, False)]
+        else:
+            calls = [varlen(ctx, tile, dt, q, k, v, False)] + ([paged(ctx, tile, dt, q, k, v, cut=100)] if at < m - n else [])
+        others = [c for c in range(d) if c not in (1, 6, 17, 40, 63)]
+        for _, got in calls:
+            assert np.all(np.isposinf(got[:, :, 1])) and np.all(np.isneginf(got[:, :, 6])) and np.all(np.isneginf(got[:, :, 63]))
+            assert np.all(np.isnan(got[:, :, 17])) and np.all(np.isnan(got[:, :, 40]))
+            o, a, size, inv = S.attend(q, k, finite, S.scalar(d, dt)[1], False)
+            if len(calls) > 1 and got is calls[1][1]:
+                o, a, size, inv = S.attend(q, k, finite, S.scalar(d, dt)[1], True)
+            S.assert_attention(got[:, :, others], (o[:, :, others], a[:, :, others], size, inv), dt, m, np.abs(finite).max(), d, f"{m} keys, one at {at}")
