@@ -147,7 +147,9 @@ __global__ __launch_bounds__(PLAN_NT) void paged_plan_kernel(const int *__restri
                     page = q < held ? table[(long)lo * p.width + q] : free_pages[first[lo] + q - held];
                     col = q;
                 }
-                slot[k] = page * p.page.d + (pos - q * p.page.d);
+                // (a page that is none, or whose slot 32 bits do not hold, gives no slot: wrapped around it would be another token's)
+                const long at_slot = (long)page * p.page.d + (pos - q * p.page.d);
+                slot[k] = at_slot >= 0 && at_slot <= 0x7FFFFFFF ? (int)at_slot : -1;
             }
         }
         if (p.wide && t0 + 4 <= p.capacity) {

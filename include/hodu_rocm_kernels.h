@@ -302,7 +302,8 @@ int hodu_rocm_attention_masked(hodu_rocm_ctx *ctx, int dtype, const void *q, con
  * added[r] new ones: the pages it lacks are taken from free_pages[0 .. n_free), in the order of the requests, and
  * entered into table[r][held ..] (held = ceil(cached / page_size); the row's other entries stay as they are); lens[r] =
  * cached + added; offsets[0 .. batch] = the new tokens' running count, which is where each request's rows begin among
- * the packed new tokens; slots[t] = where new token t is to be stored, -1 from the last token up to `capacity`;
+ * the packed new tokens; slots[t] = where new token t is to be stored, -1 from the last token up to `capacity` and for a
+ * token whose page number is negative or leads beyond 32-bit slots;
  * used[0] = pages taken (always the first of the list), used[1] = requests refused.  A request is refused -- it adds
  * no token, takes no page, and lens[r] is what was cached (0 if that is negative) -- when a length is negative, when it outgrows `width`
  * pages, when the list holds too few pages for it, or when its tokens pass `capacity`; the list and the capacity are
