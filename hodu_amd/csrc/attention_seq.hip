@@ -41,6 +41,8 @@ struct DevSeq {
 };
 
 __device__ __forceinline__ int quot(int n, const FixedDiv &f) { return fixed_quotient(n, f); }
+// keys 0 .. this that token `tok` of n attends of m, causal; <= 0: none.  (In this order no step leaves 31 bits.)
+__device__ __forceinline__ int attended(int tok, int n, int m) { return m - (n - 1 - tok); }
 
 // inclusive running sum over the wavefront's lanes (each step one instruction: shifts by 1, 2, 4, 8 within rows of 16 lanes, then
 // each row's last lane to the next row, then lane 31 to the upper half)
@@ -262,10 +264,10 @@ __global__ __launch_bounds__(R16_NT) void seq_attention_r16_kernel(const uint16_
     // the lane's row; rows past the sequence's last repeat it and are not stored
     const int rr = row0 + r < rows ? row0 + r : rows - 1;
     const int tok = quot(rr, a.by_group), head = kvh * a.group + rr - tok * a.group;
-    const int open = a.causal ? tok + m - n + 1 : m;  // keys the row attends, <= 0: none
+    const int open = a.causal ? attended(tok, n, m) : m;  // keys the row attends, <= 0: none
     const int last_tok = quot(row0 + R16 - 1 < rows ? row0 + R16 - 1 : rows - 1, a.by_group), first_tok = quot(row0, a.by_group);
-    const int keys = a.causal ? last_tok + m - n + 1 : m;          // keys the tile needs
-    const int all_open = a.causal ? first_tok + m - n + 1 : m;     // keys below this are open to every row
+    const int keys = a.causal ? attended(last_tok, n, m) : m;          // keys the tile needs
+    const int all_open = a.causal ? attended(first_tok, n, m) : m;     // keys below this are open to every row
     const int blocks = keys > 0 ? (keys + R16_BK - 1) / R16_BK : 0;
     // the tile's workgroups: as many as the launch has for it and the keys are worth
     const int worth = (blocks + R16_MIN_BLOCKS - 1) / R16_MIN_BLOCKS;
@@ -609,17 +611,17 @@ __global__ __launch_bounds__(W_NT, 1) void seq_attention_wide_kernel(const uint1
     for (int x = 0; x < RT; x++) {
         const int row = wrow0 + 16 * x + r, rr = row < rows ? row : rows - 1;
         const int tok = quot(rr, a.by_group), head = kvh * a.group + rr - tok * a.group;
-        open[x] = a.causal ? tok + m - n + 1 : m;  // keys the row attends, <= 0: none
+        open[x] = a.causal ? attended(tok, n, m) : m;  // keys the row attends, <= 0: none
         const uint16_t *q = Q + (q0 + tok) * a.q_token + head * a.q_head;
 #pragma unroll
         for (int ks = 0; ks < KS; ks++) qf[x][ks] = *reinterpret_cast<const u32x4_t *>(q + 32 * ks + 8 * g);
     }
     const float c = exponent_scale(a.scale_log2e * (F8 ? a.k_scale[kvh] : 1.f));
     auto last_row = [&](int i) { return i < rows ? i : rows - 1; };
-    const int keys_any = a.causal ? quot(last_row(row0 + BM - 1), a.by_group) + m - n + 1 : m;  // keys the tile needs
+    const int keys_any = a.causal ? attended(quot(last_row(row0 + BM - 1), a.by_group), n, m) : m;  // keys the tile needs
     int keys = keys_any > 0 ? keys_any : 0;
-    int wave_keys = a.causal ? quot(last_row(wrow0 + 16 * RT - 1), a.by_group) + m - n + 1 : m;  // ... the wavefront needs
-    int all_open = a.causal ? quot(last_row(wrow0), a.by_group) + m - n + 1 : m;  // keys below this are open to all its rows
+    int wave_keys = a.causal ? attended(quot(last_row(wrow0 + 16 * RT - 1), a.by_group), n, m) : m;  // ... the wavefront needs
+    int all_open = a.causal ? attended(quot(last_row(wrow0), a.by_group), n, m) : m;  // keys below this are open to all its rows
     int stages = (keys + W_BK - 1) / W_BK;
     // few tiles over a long cache: this workgroup's range of the keys, and everything from here on counts from its first one
     int from = 0, splits = 1;

@@ -236,6 +236,8 @@ int parse_attention_metadata(const size_t *md, size_t len, AttentionArgs *a) {
 
 namespace {
 constexpr size_t kMaxInt = 0x7FFFFFFF;
+// rows of a sequence and key / value head, and keys of a sequence: a tile's counting past the last of either stays below 2^31
+constexpr size_t kMaxCount = kMaxInt - 4095;
 // a metadata vector of exactly `want` words, each in range
 int check_words(const char *what, const size_t *md, size_t len, size_t want) {
     if (!md) return fail(HODU_ROCM_INVALID_ARG, "%s: metadata is null", what);
@@ -252,12 +254,12 @@ int check_pages(const char *what, size_t pages, size_t page_size, const char *of
     return HODU_ROCM_OK;
 }
 int check_heads(const char *what, size_t batch, size_t tokens, size_t heads, size_t kv_heads) {
-    if (batch > kMaxInt - 1 || tokens > kMaxInt || heads > kMaxInt || kv_heads > kMaxInt)
-        return fail(HODU_ROCM_UNSUPPORTED, "%s: more than 2^31 - 1 sequences, tokens or heads", what);
+    if (batch > kMaxCount || tokens > kMaxCount || heads > kMaxInt || kv_heads > kMaxInt)
+        return fail(HODU_ROCM_UNSUPPORTED, "%s: more than 2^31 - 4096 sequences or tokens, or 2^31 - 1 heads", what);
     if (kv_heads < 1 || heads < 1 || heads % kv_heads)
         return fail(HODU_ROCM_INVALID_ARG, "%s: %zu heads do not share %zu key / value heads evenly", what, heads, kv_heads);
-    if (tokens * (heads / kv_heads) > kMaxInt)
-        return fail(HODU_ROCM_UNSUPPORTED, "%s: %zu tokens of %zu heads per key / value head exceed 2^31 - 1 rows", what, tokens, heads / kv_heads);
+    if (tokens * (heads / kv_heads) > kMaxCount)
+        return fail(HODU_ROCM_UNSUPPORTED, "%s: %zu tokens of %zu heads per key / value head exceed 2^31 - 4096 rows", what, tokens, heads / kv_heads);
     return HODU_ROCM_OK;
 }
 }  // namespace
@@ -295,7 +297,7 @@ int parse_paged_store_metadata(const size_t *md, size_t len, PagedStoreArgs *a) 
 int parse_varlen_metadata(const size_t *md, size_t len, SeqAttentionArgs *a) {
     if (int rc = check_words("attention_varlen", md, len, 15)) return rc;
     if (int rc = check_heads("attention_varlen", md[0], md[1], md[3], md[4])) return rc;
-    if (md[2] > kMaxInt) return fail(HODU_ROCM_UNSUPPORTED, "attention_varlen: more than 2^31 - 1 keys");
+    if (md[2] > kMaxCount) return fail(HODU_ROCM_UNSUPPORTED, "attention_varlen: more than 2^31 - 4096 keys");
     *a = SeqAttentionArgs{};
     a->batch = (long)md[0]; a->q_tokens = (long)md[1]; a->k_tokens = (long)md[2];
     a->heads = (long)md[3]; a->kv_heads = (long)md[4]; a->d = (long)md[5];
@@ -313,6 +315,7 @@ int parse_paged_attention_metadata(const size_t *md, size_t len, SeqAttentionArg
     if (int rc = check_heads("attention_paged", md[0], md[1], md[2], md[3])) return rc;
     if (int rc = check_pages("attention_paged", md[5], md[6], "the cache")) return rc;
     if (int rc = check_pages("attention_paged", md[7], md[6], "a table row")) return rc;
+    if (md[7] * md[6] > kMaxCount) return fail(HODU_ROCM_UNSUPPORTED, "attention_paged: a table row of more than 2^31 - 4096 keys");
     *a = SeqAttentionArgs{};
     a->paged = true;
     a->causal = true;

@@ -336,7 +336,8 @@ int hodu_rocm_paged_store(hodu_rocm_ctx *ctx, int dtype, int cache_dtype, const 
  * the row NaN although the row does not attend it (zero times infinity), values of other sequences never do.  An infinite
  * value that a row attends makes its column infinite, unless the key's probability rounds to zero in `dtype` (NaN).
  * dtype: bf16 or f16; D = 64 or 128; the D elements dense, strides and offsets multiples of 8 elements, bases of 16
- * bytes; scale: the scalar in `dtype`, positive and finite.  HODU_ROCM_UNSUPPORTED otherwise.
+ * bytes; scale: the scalar in `dtype`, positive and finite; sequences, keys (paged: of a table row) and rows per key / value head
+ * up to 2^31 - 4096.  HODU_ROCM_UNSUPPORTED otherwise.
  * metadata: [batch, q_tokens, k_tokens, heads, kv_heads, D, q_token, q_head, k_token, k_head, v_token, v_head, q_off,
  * k_off, v_off] (element strides between tokens and heads). */
 int hodu_rocm_attention_varlen(hodu_rocm_ctx *ctx, int dtype, const void *q, const void *k, const void *v, void *out,
