@@ -995,12 +995,13 @@ __global__ __launch_bounds__(W_NT, 1) void seq_attention_wide_kernel(const uint1
             for (int ks = 0; ks < KS; ks++) mfma::pin_accumulation(qf[x][ks]);
         __syncthreads();
         int st = 0;
-        auto begin_stage = [&]() __attribute__((always_inline)) {
+        // may_end: the stage may be the tile's last
+        auto begin_stage = [&](auto may_end) __attribute__((always_inline)) {
             // K of stage st + 1 and V of stage st have landed (what was issued at the last stage may be in flight), everybody's;
             // and everybody is done with what this stage's loads overwrite
             if (st > 0 && st + 2 < stages) __builtin_amdgcn_s_waitcnt(mfma::waitcnt_vm_lgkm0(2 * G::NI));
             else __builtin_amdgcn_s_waitcnt(mfma::waitcnt_vm_lgkm0(0));
-            if constexpr (!F8) {
+            if constexpr (!F8 && decltype(may_end)::value) {
                 // the copies of the last key, which P is zero of: an infinite value times zero would be a NaN.  (Each wavefront its own,
                 // which have landed; 8-bit values have no infinity.)
                 if ((st + 1) * W_BK > keys) {
@@ -1047,8 +1048,8 @@ __global__ __launch_bounds__(W_NT, 1) void seq_attention_wide_kernel(const uint1
                 first_fragments(k_of(2 * st + 1));
                 bool half = false;
                 if ((2 * st + 3) * 32 <= all_open) {
-                    do {
-                        begin_stage();
+                    do {  // (keys follow that are open to all rows)
+                        begin_stage(std::false_type());
                         step(std::false_type(), std::false_type(), 2 * st, sc, sn, pc, pn);
                         if (some_exceed()) { half = true; break; }
                         step(std::false_type(), std::true_type(), 2 * st + 1, sn, sc, pn, pc);
@@ -1056,7 +1057,7 @@ __global__ __launch_bounds__(W_NT, 1) void seq_attention_wide_kernel(const uint1
                     } while (!some_exceed() && (2 * st + 3) * 32 <= all_open);
                 } else {
                     do {
-                        begin_stage();
+                        begin_stage(std::true_type());
                         step(std::true_type(), std::false_type(), 2 * st, sc, sn, pc, pn);
                         if (some_exceed()) { half = true; break; }
                         step(std::true_type(), std::true_type(), 2 * st + 1, sn, sc, pn, pc);
@@ -1073,7 +1074,7 @@ __global__ __launch_bounds__(W_NT, 1) void seq_attention_wide_kernel(const uint1
                     }
                 }
             } else {
-                if (!(i & 1)) begin_stage();
+                if (!(i & 1)) begin_stage(std::true_type());
                 if (i <= steps) slow_step(i, sc, pc);
                 if constexpr (PAGED)
                     if (i & 1)
