@@ -273,6 +273,14 @@ def _words(md: Sequence[int]):
     return (ctypes.c_size_t * len(md))(*md), len(md)
 
 
+def _scale_word(dt: str, scale):
+    """attention's scale as the library reads it: one element in dt's storage (a float64's first two bytes are another number)"""
+    sc = np.ascontiguousarray(scale).reshape(1)
+    if sc.itemsize != DTYPE_SIZE[dt]:
+        raise HoduRocmError(INVALID_ARG, f"scale: one element in the storage of {dt} is needed, got {sc.dtype}")
+    return sc
+
+
 class DeviceBuffer:
     """A device allocation owned by a Context (what CudaSlice is to the CUDA sibling)."""
 
@@ -533,7 +541,7 @@ class Context:
             if n_out * DTYPE_SIZE[dt] > out.nbytes:
                 raise HoduRocmError(INVALID_ARG, "attention: the output buffer is too small")
         arr, n = _md_array(md)
-        sc = np.ascontiguousarray(scale).reshape(1)
+        sc = _scale_word(dt, scale)
         if mask is not None:
             strides = [int(x) for x in mask_strides]
             if len(m) != 1 + nb + 3 + 3 * (nb + 2) + 3 or len(strides) != nb + 2:
@@ -590,7 +598,7 @@ class Context:
                     ("v", v, _span3(tk, hk, d, vt, vh, vo) * es), ("out", out, tq * hq * d * es), ("q_offsets", q_offsets, 4 * b + 4),
                     ("k_offsets", k_offsets, 4 * b + 4))
         arr, n = _words(md)
-        sc = np.ascontiguousarray(scale).reshape(1)
+        sc = _scale_word(dt, scale)
         self._check(self.lib.hodu_rocm_attention_varlen(self.handle, DTYPE_ID[dt], q.ptr, k.ptr, v.ptr, out.ptr, q_offsets.ptr,
                                                         k_offsets.ptr, arr, n, sc.ctypes.data, int(bool(causal))))
 
@@ -611,7 +619,7 @@ class Context:
                 if buf is not None:
                     _within("attention_paged", (name, buf, 4 * hk))
         arr, n = _words(md)
-        sc = np.ascontiguousarray(scale).reshape(1)
+        sc = _scale_word(dt, scale)
         self._check(self.lib.hodu_rocm_attention_paged(
             self.handle, DTYPE_ID[dt], DTYPE_ID[cache_dt], q.ptr, k_cache.ptr, v_cache.ptr, out.ptr, q_offsets.ptr, table.ptr, lens.ptr,
             None if k_scale is None else k_scale.ptr, None if v_scale is None else v_scale.ptr, arr, n, sc.ctypes.data))

@@ -1,0 +1,37 @@
+"""What the Python binding refuses before a call reaches the library (CPU build of the kernels, tests/emu_util.EmuContext): a scale
+that is not in the operands' storage."""
+import numpy as np
+import pytest
+
+import emu_util
+import seq_util as S
+from hodu_amd import ffi
+
+pytestmark = pytest.mark.skipif(emu_util.compiler() is None, reason="no host clang++ for the CPU build")
+
+
+@pytest.fixture()
+def ctx():
+    c = emu_util.EmuContext()
+    yield c
+    c.close()
+
+
+def attentions(ctx, view=lambda b: b):
+    """{name: call(scale)} of the attention entry points on small operands; view: wraps the first operand"""
+    d, n = 64, 4
+    q, k, v, out = (ctx.upload(np.zeros(n * d, np.uint16)) for _ in range(4))
+    off, table, lens = ctx.upload(np.array([0, n], np.int32)), ctx.upload(np.zeros((1, 1), np.int32)), ctx.upload(np.array([n], np.int32))
+    dense = (1, 1, n, n, d, n * d, d, 1, n * d, d, 1, n * d, d, 1, 0, 0, 0)
+    return {"attention": lambda scale: ctx.attention("bf16", view(q), k, v, out, dense, scale),
+            "attention_varlen": lambda scale: ctx.attention_varlen("bf16", view(q), k, v, out, off, off, ffi.varlen_md(1, n, n, 1, 1, d), scale),
+            "attention_paged": lambda scale: ctx.attention_paged("bf16", view(q), k, v, out, off, table, lens, ffi.paged_attention_md(1, n, 1, 1, d, 1, n, 1), scale)}
+
+
+@pytest.mark.parametrize("name", ["attention", "attention_varlen", "attention_paged"])
+def test_a_scale_of_another_storage_is_refused(ctx, name):
+    call = attentions(ctx)[name]
+    call(S.scalar(64, "bf16")[0])
+    for scale in (0.125, np.float32(0.125), np.array([0.125]), np.zeros(1, np.uint8), np.zeros(2, np.uint16)):
+        with pytest.raises((ffi.HoduRocmError, ValueError)):
+            call(scale)
