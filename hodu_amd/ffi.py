@@ -256,11 +256,13 @@ def _span4(d0, d1, d2, d3, s0, s1, s2, offset):
     return offset + (d0 - 1) * s0 + (d1 - 1) * s1 + (d2 - 1) * s2 + d3 if d0 and d1 and d2 and d3 else 0
 
 
-def _within(what, *needs):
-    """refuse a launch that reaches past one of the device buffers; needs: (name, buffer, bytes)"""
+def _within(what, device, *needs):
+    """refuse a launch that reaches past one of the device buffers, or into another device's; needs: (name, buffer, bytes)"""
     for name, buf, nbytes in needs:
         if nbytes > buf.nbytes:
             raise HoduRocmError(INVALID_ARG, f"{what}: addresses {nbytes} bytes of {name} but the buffer holds {buf.nbytes}")
+        if buf.device is not None and buf.device != device:
+            raise HoduRocmError(INVALID_ARG, f"{what}: {name} is on device {buf.device}, the context on device {device}")
 
 
 def _md_array(md: Sequence[int]):
@@ -286,6 +288,7 @@ class DeviceBuffer:
 
     def __init__(self, ctx: "Context", nbytes: int):
         self.ctx = ctx
+        self.device = ctx.device
         self.nbytes = int(nbytes)
         p = ctypes.c_void_p()
         ctx._check(ctx.lib.hodu_rocm_alloc(ctx.handle, self.nbytes, ctypes.byref(p)))
@@ -307,20 +310,20 @@ class DeviceView:
     """Device memory that somebody else owns (another library's tensor, a part of a DeviceBuffer), as an operand: the
     calls that take a DeviceBuffer take one of these.  The owner keeps the memory alive, and its own work on it is in order
     with the context's calls only where they share a stream: Context.set_stream(torch.cuda.current_stream())."""
-    __slots__ = ("ptr", "nbytes")
+    __slots__ = ("ptr", "nbytes", "device")
 
-    def __init__(self, ptr: int, nbytes: int):
-        self.ptr, self.nbytes = ptr, nbytes
+    def __init__(self, ptr: int, nbytes: int, device: Optional[int] = None):
+        self.ptr, self.nbytes, self.device = ptr, nbytes, device
 
     @classmethod
     def of(cls, tensor) -> "DeviceView":
-        """of a torch tensor on the context's device: its elements or, where they do not lie side by side, all up to the end of its
+        """of a torch tensor (one on another device than the context's is refused by the call): its elements or, where they do not lie side by side, all up to the end of its
         storage"""
         if not tensor.is_cuda:
             raise ValueError(f"a tensor on the GPU is needed, got one on {tensor.device}")
         if tensor.is_contiguous():
-            return cls(tensor.data_ptr(), tensor.nbytes)
-        return cls(tensor.data_ptr(), tensor.untyped_storage().nbytes() - tensor.storage_offset() * tensor.element_size())
+            return cls(tensor.data_ptr(), tensor.nbytes, tensor.get_device())
+        return cls(tensor.data_ptr(), tensor.untyped_storage().nbytes() - tensor.storage_offset() * tensor.element_size(), tensor.get_device())
 
 
 class Context:
@@ -560,11 +563,11 @@ class Context:
         are i32 device buffers; free_pages and slots may be None where the list or the capacity is empty"""
         if len(md) == 5:
             b, _, width, n_free, capacity = md
-            _within("paged_plan", ("cached", cached, 4 * b), ("added", added, 4 * b), ("table", table, 4 * b * width), ("lens", lens, 4 * b),
+            _within("paged_plan", self.device, ("cached", cached, 4 * b), ("added", added, 4 * b), ("table", table, 4 * b * width), ("lens", lens, 4 * b),
                     ("offsets", offsets, 4 * b + 4), ("used", used, 8))
             for name, buf, n in (("free_pages", free_pages, n_free), ("slots", slots, capacity)):
                 if buf is not None:
-                    _within("paged_plan", (name, buf, 4 * n))
+                    _within("paged_plan", self.device, (name, buf, 4 * n))
         arr, n = _words(md)
         self._check(self.lib.hodu_rocm_paged_plan(
             self.handle, cached.ptr, added.ptr, None if free_pages is None else free_pages.ptr, table.ptr, lens.ptr, offsets.ptr,
@@ -577,12 +580,12 @@ class Context:
         if len(md) == 19:
             t, h, d, kt, kh, vt, vh, ko, vo, pages, page, kcp, kct, kch, vcp, vct, vch, kco, vco = md
             es, ces = DTYPE_SIZE[dt], DTYPE_SIZE[cache_dt]
-            _within("paged_store", ("k", k, _span3(t, h, d, kt, kh, ko) * es), ("v", v, _span3(t, h, d, vt, vh, vo) * es),
+            _within("paged_store", self.device, ("k", k, _span3(t, h, d, kt, kh, ko) * es), ("v", v, _span3(t, h, d, vt, vh, vo) * es),
                     ("k_cache", k_cache, _span4(pages, page, h, d, kcp, kct, kch, kco) * ces),
                     ("v_cache", v_cache, _span4(pages, page, h, d, vcp, vct, vch, vco) * ces), ("slots", slots, 4 * t))
             for name, buf in (("k_scale", k_scale), ("v_scale", v_scale)):
                 if buf is not None:
-                    _within("paged_store", (name, buf, 4 * h))
+                    _within("paged_store", self.device, (name, buf, 4 * h))
         arr, n = _words(md)
         self._check(self.lib.hodu_rocm_paged_store(
             self.handle, DTYPE_ID[dt], DTYPE_ID[cache_dt], k.ptr, v.ptr, k_cache.ptr, v_cache.ptr, slots.ptr,
@@ -594,7 +597,7 @@ class Context:
         if len(md) == 15:
             b, tq, tk, hq, hk, d, qt, qh, kt, kh, vt, vh, qo, ko, vo = md
             es = DTYPE_SIZE[dt]
-            _within("attention_varlen", ("q", q, _span3(tq, hq, d, qt, qh, qo) * es), ("k", k, _span3(tk, hk, d, kt, kh, ko) * es),
+            _within("attention_varlen", self.device, ("q", q, _span3(tq, hq, d, qt, qh, qo) * es), ("k", k, _span3(tk, hk, d, kt, kh, ko) * es),
                     ("v", v, _span3(tk, hk, d, vt, vh, vo) * es), ("out", out, tq * hq * d * es), ("q_offsets", q_offsets, 4 * b + 4),
                     ("k_offsets", k_offsets, 4 * b + 4))
         arr, n = _words(md)
@@ -611,13 +614,13 @@ class Context:
         if len(md) == 19:
             b, tq, hq, hk, d, pages, page, width, qt, qh, qo, kcp, kct, kch, vcp, vct, vch, kco, vco = md
             es, ces = DTYPE_SIZE[dt], DTYPE_SIZE[cache_dt]
-            _within("attention_paged", ("q", q, _span3(tq, hq, d, qt, qh, qo) * es),
+            _within("attention_paged", self.device, ("q", q, _span3(tq, hq, d, qt, qh, qo) * es),
                     ("k_cache", k_cache, _span4(pages, page, hk, d, kcp, kct, kch, kco) * ces),
                     ("v_cache", v_cache, _span4(pages, page, hk, d, vcp, vct, vch, vco) * ces), ("out", out, tq * hq * d * es),
                     ("q_offsets", q_offsets, 4 * b + 4), ("table", table, 4 * b * width), ("lens", lens, 4 * b))
             for name, buf in (("k_scale", k_scale), ("v_scale", v_scale)):
                 if buf is not None:
-                    _within("attention_paged", (name, buf, 4 * hk))
+                    _within("attention_paged", self.device, (name, buf, 4 * hk))
         arr, n = _words(md)
         sc = _scale_word(dt, scale)
         self._check(self.lib.hodu_rocm_attention_paged(
