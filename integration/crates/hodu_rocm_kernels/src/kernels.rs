@@ -155,3 +155,84 @@ pub fn call_ops_attention(ctx: &Context, dtype: u8, q: &DeviceBuf, k: &DeviceBuf
         Err(e) => Err(e),
     }
 }
+
+/// A cache of keys and values in 8 bits: f8e4m3 with one f32 scale per key / value head, on the device.  `None` in its
+/// place: a cache in the operands' dtype.
+pub struct CacheScales<'a> {
+    pub k: &'a DeviceBuf,
+    pub v: &'a DeviceBuf,
+}
+
+// the cache's dtype (hodu's discriminant of F8E4M3, or the operands' own) and its scales as the library takes them
+fn cache_args(dtype: u8, scales: &Option<CacheScales>) -> (c_int, *const f32, *const f32) {
+    const F8E4M3: c_int = 1;
+    match scales {
+        None => (dtype as c_int, core::ptr::null(), core::ptr::null()),
+        Some(s) => (F8E4M3, s.k.as_ptr() as *const f32, s.v.as_ptr() as *const f32),
+    }
+}
+
+/// What call_ops_paged_plan fills, all of it i32 on the device: `table` [batch, width], `lens` [batch], `offsets`
+/// [batch + 1], `slots` [capacity], `used` [2].
+pub struct PagedPlan<'a> {
+    pub table: &'a DeviceBuf,
+    pub lens: &'a DeviceBuf,
+    pub offsets: &'a DeviceBuf,
+    pub slots: &'a DeviceBuf,
+    pub used: &'a DeviceBuf,
+}
+
+/// Block tables and slot maps of a paged cache from request lengths (`cached`, `added`: i32, batch each; `free_pages`:
+/// i32); metadata = [batch, page_size, width, n_free, capacity].
+pub fn call_ops_paged_plan(ctx: &Context, cached: &DeviceBuf, added: &DeviceBuf, free_pages: &DeviceBuf, plan: &PagedPlan,
+                           metadata: &[usize]) -> Result<()> {
+    ctx.check(unsafe {
+        ffi::hodu_rocm_paged_plan(ctx.raw(), cached.as_ptr() as *const c_int, added.as_ptr() as *const c_int,
+                                  free_pages.as_ptr() as *const c_int, plan.table.as_mut_ptr() as *mut c_int,
+                                  plan.lens.as_mut_ptr() as *mut c_int, plan.offsets.as_mut_ptr() as *mut c_int,
+                                  plan.slots.as_mut_ptr() as *mut c_int, plan.used.as_mut_ptr() as *mut c_int,
+                                  metadata.as_ptr(), metadata.len())
+    })
+}
+
+/// New keys and values into their slots of the cache; metadata = [tokens, kv_heads, D, k_token, k_head, v_token, v_head,
+/// k_off, v_off, n_pages, page_size, k cache strides (page, token, head), v cache strides, k_cache_off, v_cache_off].
+pub fn call_ops_paged_store(ctx: &Context, dtype: u8, k: &DeviceBuf, v: &DeviceBuf, k_cache: &DeviceBuf, v_cache: &DeviceBuf,
+                            slots: &DeviceBuf, scales: Option<CacheScales>, metadata: &[usize]) -> Result<()> {
+    let (cache_dtype, k_scale, v_scale) = cache_args(dtype, &scales);
+    ctx.check(unsafe {
+        ffi::hodu_rocm_paged_store(ctx.raw(), dtype as c_int, cache_dtype, k.as_ptr(), v.as_ptr(), k_cache.as_mut_ptr(),
+                                   v_cache.as_mut_ptr(), slots.as_ptr() as *const c_int, k_scale, v_scale, metadata.as_ptr(),
+                                   metadata.len())
+    })
+}
+
+/// Attention over packed sequences of different lengths with grouped heads; `q_offsets`, `k_offsets`: i32, batch + 1
+/// each; `scale`: the scalar in `dtype`'s storage; metadata = [batch, q_tokens, k_tokens, heads, kv_heads, D, q_token,
+/// q_head, k_token, k_head, v_token, v_head, q_off, k_off, v_off].  There is no other route to fall back to, so a call
+/// that the kernels do not take is an error.
+pub fn call_ops_attention_varlen(ctx: &Context, dtype: u8, q: &DeviceBuf, k: &DeviceBuf, v: &DeviceBuf, out: &DeviceBuf,
+                                 q_offsets: &DeviceBuf, k_offsets: &DeviceBuf, metadata: &[usize], scale: [u8; 2],
+                                 causal: bool) -> Result<()> {
+    ctx.check(unsafe {
+        ffi::hodu_rocm_attention_varlen(ctx.raw(), dtype as c_int, q.as_ptr(), k.as_ptr(), v.as_ptr(), out.as_mut_ptr(),
+                                        q_offsets.as_ptr() as *const c_int, k_offsets.as_ptr() as *const c_int,
+                                        metadata.as_ptr(), metadata.len(), scale.as_ptr() as *const core::ffi::c_void,
+                                        causal as c_int)
+    })
+}
+
+/// Attention of each request's last tokens over its pages of the cache; `q_offsets` [batch + 1], `table` [batch, width],
+/// `lens` [batch]: i32; metadata = [batch, q_tokens, heads, kv_heads, D, n_pages, page_size, width, q_token, q_head,
+/// q_off, k cache strides (page, token, head), v cache strides, k_cache_off, v_cache_off].
+pub fn call_ops_attention_paged(ctx: &Context, dtype: u8, q: &DeviceBuf, k_cache: &DeviceBuf, v_cache: &DeviceBuf,
+                                out: &DeviceBuf, q_offsets: &DeviceBuf, table: &DeviceBuf, lens: &DeviceBuf,
+                                scales: Option<CacheScales>, metadata: &[usize], scale: [u8; 2]) -> Result<()> {
+    let (cache_dtype, k_scale, v_scale) = cache_args(dtype, &scales);
+    ctx.check(unsafe {
+        ffi::hodu_rocm_attention_paged(ctx.raw(), dtype as c_int, cache_dtype, q.as_ptr(), k_cache.as_ptr(), v_cache.as_ptr(),
+                                       out.as_mut_ptr(), q_offsets.as_ptr() as *const c_int, table.as_ptr() as *const c_int,
+                                       lens.as_ptr() as *const c_int, k_scale, v_scale, metadata.as_ptr(), metadata.len(),
+                                       scale.as_ptr() as *const core::ffi::c_void)
+    })
+}
