@@ -116,7 +116,9 @@ template <int ROWS, bool PAGED> __device__ __forceinline__ bool find_tile(const 
 // The same for tiles that work for long, of up to 64 sequences: the ones with most keys first and each from its last row, so that
 // the tiles left over at a launch's end are short ones (in the sequences' own order and with it: 8192 tokens 679 and 594 us, four chunks of
 // 512 over up to 8192 390 and 361, 64 single tokens over up to 8192 270 and 254, 16 packed prompts 421 and 413).  Above 64, one sequence a
-// lane does not do, and a launch has rounds enough to even out.  A lane owns a sequence, sums the tiles of those before it in that order, and
+// lane does not do, and the sequences' own order is taken: the same requests with an empty one more than 64 cost, this order and that, 255
+// and 286 us (64 single tokens over up to 8192), 81 and 88 (over up to 2048), 175 and 185 (64 chunks of 64), but 661 and 612 (64 prompts of up
+// to 1024).  A lane owns a sequence, sums the tiles of those before it in that order, and
 // knows whether the tile is its own.
 template <int ROWS, bool PAGED> __device__ __forceinline__ bool find_tile_long_first(const DevSeq &a, int tile, SeqTile &f) {
     const int lane = threadIdx.x & 63, s = lane < a.batch ? lane : a.batch - 1;
@@ -175,9 +177,9 @@ template <int CK> __device__ __forceinline__ u32x4_t widen8(const u32x2_t &v) {
 // rows; the keys of a tile are cut into ranges of 32-key blocks, one per wavefront of each of the tile's workgroups, so that a single long
 // sequence still reaches every compute unit.  A wavefront has an LDS ring of its own (32 KB: the next block or blocks are in flight while it computes,
 // 64 KB and more per compute unit), meets nobody until its range is done, and there is no barrier in the loop.
-// Measured, bf16, 32 query and 8 key / value heads of 128: 64 tokens over up to 8192 cached each, 1.44 GB, 253 us (5.7 TB/s; a
+// Measured, bf16, 32 query and 8 key / value heads of 128: 64 tokens over up to 8192 cached each, 1.44 GB, 255 us (5.6 TB/s; a
 // large copy 5.1, reading alone 7.0); 48 over up to 16384 in 8-bit floats, 64 query heads, 1.08 GB, 230 us (4.7 TB/s: what a workgroup
-// costs besides its keys, three rounds of it; eight wavefronts with half the ring each 227); one over 1999, 8 MB, 10.6 us.
+// costs besides its keys, three rounds of it; eight wavefronts with half the ring each 227); one over 1999, 8 MB, 11.5 us.
 //
 // S^T = K Q^T and O^T += V^T P^T on 16 x 16 x 32: a lane then owns one row throughout (column lane % 16).  The rows
 // of the first product's left operand are keys in the order 8 (r / 4) + 4 t + r % 4 for tile t of two, so that a lane's
@@ -544,9 +546,13 @@ __global__ __launch_bounds__(R16_NT) void seq_attention_r16_kernel(const uint16_
 // rows each (RT = 2, 3 or 4 tiles of 16) and walk all keys of the tile, 64 to a stage of the LDS ring, 32 to a step, with the layouts of the
 // kernel above.  A fragment of K or V read from LDS feeds RT matrix instructions, which is what keeps LDS from being the bound
 // (128 bytes a cycle: a fragment per 2 RT cycles of each SIMD; the instruction takes 16).
-// Measured, bf16, causal, 32 query and 8 key / value heads of 128: 8192 tokens 543 us (1012 TFLOP/s; a matrix product of 8192^3 runs
-// at 1210); 16 prompts of up to 2048 tokens 382 us (642: a workgroup costs some 10 us besides its stages of 1.5 us, and a tile of
-// those has 10 of them); four chunks of 512 tokens over up to 8192 287 us (753).
+// Measured, bf16, causal, 32 query and 8 key / value heads of 128: 8192 tokens 547 us (1004 TFLOP/s; a matrix product of 8192^3 runs
+// at 1210); 16 prompts of up to 2048 tokens 390 us (629: a workgroup costs some 10 us besides its stages of 1.5 us, and a tile of
+// those has 10 of them); four chunks of 512 tokens over up to 8192 285 us (758).
+//
+// P is rounded to the type for the second product, and the row sum is taken of it as rounded: the output is off by 1.3 to 1.4 times
+// what its own rounding costs.  What the rounding leaves could be multiplied too, as the kernel above does where memory is the bound;
+// here it would be 27 more matrix instructions to a step of 51 (head dim 128, three tiles), and they are the bound.
 //
 // A wavefront issues in order, an instruction every 4 cycles, and a matrix instruction runs for 16: the exponentials have
 // to stand BETWEEN the matrix instructions.  So a step holds three independent pieces of work -- scores of step i + 1,

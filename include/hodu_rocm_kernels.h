@@ -357,7 +357,8 @@ int hodu_rocm_attention_varlen(hodu_rocm_ctx *ctx, int dtype, const void *q, con
  * which may have to grow (not with the rows: fewer of them are cut into more ranges).  It cannot grow while the stream is
  * being captured -- such a call is refused with HODU_ROCM_SCRATCH: run it once, with the same sizes, before capturing it.
  * A graph keeps the workspace it was captured with for as long as the context lives, also when later calls need a larger
- * one; replay graphs captured from one context one after the other. */
+ * one; replay graphs captured from one context one after the other, and not beside the context's own calls (on the
+ * stream that they are issued on, which orders both). */
 int hodu_rocm_attention_paged(hodu_rocm_ctx *ctx, int dtype, int cache_dtype, const void *q, const void *k_cache,
                               const void *v_cache, void *out, const int *q_offsets, const int *table, const int *lens,
                               const float *k_scale, const float *v_scale, const size_t *metadata, size_t metadata_len,
