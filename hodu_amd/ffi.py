@@ -399,7 +399,9 @@ class Context:
     def set_stream(self, stream):
         """hodu_rocm_ctx_set_stream: issue every later call on `stream` -- a hipStream_t as a number (0: the default stream) or
         an object that has one as cuda_stream, as torch's streams do -- behind what the context issued before.  The
-        stream has to stay alive until another one is set or the context closed"""
+        stream has to stay alive until another one is set or the context closed.  torch has to be imported before this
+        library is loaded (the first Context): it brings a HIP runtime of its own, which the library then shares, while torch
+        finds no GPU in a process that has loaded another runtime first"""
         handle = int(getattr(stream, "cuda_stream", stream))
         if handle != self._stream:
             self._check(self.lib.hodu_rocm_ctx_set_stream(self.handle, handle))
