@@ -23,6 +23,7 @@ constexpr int PLAN_MAX_BATCH = 8192;  // 12 bytes of LDS each
 
 struct DevPlan {
     int batch, width, n_free, capacity;
+    int most_pages;  // that 32-bit slots number
     FixedDiv page;
     int wide;  // slots are 16-byte aligned
 };
@@ -135,7 +136,7 @@ __global__ __launch_bounds__(PLAN_NT) void paged_plan_kernel(const int *__restri
                 const int mid = (lo + hi + 1) >> 1;
                 if (at[mid] <= t0) lo = mid; else hi = mid - 1;
             }
-            int col = -1, page = 0;
+            int col = -1, first_slot = 0;
 #pragma unroll
             for (int k = 0; k < 4; k++) {
                 const int t = (int)t0 + k;
@@ -144,12 +145,12 @@ __global__ __launch_bounds__(PLAN_NT) void paged_plan_kernel(const int *__restri
                 const int pos = had[lo] + (t - at[lo]), q = fixed_quotient(pos, p.page);
                 if (q != col) {
                     const int held = fixed_quotient(had[lo], p.page) + (fixed_quotient(had[lo], p.page) * p.page.d < had[lo] ? 1 : 0);
-                    page = q < held ? table[(long)lo * p.width + q] : free_pages[first[lo] + q - held];
+                    const int page = q < held ? table[(long)lo * p.width + q] : free_pages[first[lo] + q - held];
+                    // (a page that is none, or whose slots 32 bits do not hold, gives no slot: wrapped around it would be another token's)
+                    first_slot = (unsigned)page < (unsigned)p.most_pages ? page * p.page.d : -1;
                     col = q;
                 }
-                // (a page that is none, or whose slot 32 bits do not hold, gives no slot: wrapped around it would be another token's)
-                const long at_slot = (long)page * p.page.d + (pos - q * p.page.d);
-                slot[k] = at_slot >= 0 && at_slot <= 0x7FFFFFFF ? (int)at_slot : -1;
+                slot[k] = first_slot < 0 ? -1 : first_slot + (pos - q * p.page.d);
             }
         }
         if (p.wide && t0 + 4 <= p.capacity) {
@@ -228,6 +229,7 @@ int launch_paged_plan(hodu_rocm_ctx *ctx, const int *cached, const int *added, c
     if (a.batch > PLAN_MAX_BATCH) return fail(HODU_ROCM_UNSUPPORTED, "paged_plan: at most %d requests, got %ld", PLAN_MAX_BATCH, a.batch);
     DevPlan p{};
     p.batch = (int)a.batch; p.width = (int)a.width; p.n_free = (int)a.n_free; p.capacity = (int)a.capacity;
+    p.most_pages = (int)((1L << 31) / a.page_size < 0x7FFFFFFF ? (1L << 31) / a.page_size : 0x7FFFFFFF);
     p.page = fixed_div((int)a.page_size);
     p.wide = (uintptr_t)slots % 16 == 0;
     const int lds = (int)(20 + 3 * a.batch + 1) * 4;
