@@ -261,7 +261,7 @@ def _within(what, device, *needs):
     for name, buf, nbytes in needs:
         if nbytes > buf.nbytes:
             raise HoduRocmError(INVALID_ARG, f"{what}: addresses {nbytes} bytes of {name} but the buffer holds {buf.nbytes}")
-        if buf.device is not None and buf.device != device:
+        if buf.device != device and buf.device is not None:
             raise HoduRocmError(INVALID_ARG, f"{what}: {name} is on device {buf.device}, the context on device {device}")
 
 
@@ -319,11 +319,12 @@ class DeviceView:
     def of(cls, tensor) -> "DeviceView":
         """of a torch tensor (one on another device than the context's is refused by the call): its elements or, where they do not lie side by side, all up to the end of its
         storage"""
-        if not tensor.is_cuda:
+        device = tensor.get_device()  # (-1: none)
+        if device < 0:
             raise ValueError(f"a tensor on the GPU is needed, got one on {tensor.device}")
         if tensor.is_contiguous():
-            return cls(tensor.data_ptr(), tensor.nbytes, tensor.get_device())
-        return cls(tensor.data_ptr(), tensor.untyped_storage().nbytes() - tensor.storage_offset() * tensor.element_size(), tensor.get_device())
+            return cls(tensor.data_ptr(), tensor.nbytes, device)
+        return cls(tensor.data_ptr(), tensor.untyped_storage().nbytes() - tensor.storage_offset() * tensor.element_size(), device)
 
 
 class Context:

@@ -41,7 +41,7 @@ class Tensor:
     """what DeviceView.of reads of a torch tensor"""
 
     def __init__(self, buf, index):
-        self.is_cuda, self.nbytes, self.buf, self.index = True, buf.nbytes, buf, index
+        self.nbytes, self.buf, self.index = buf.nbytes, buf, index
 
     def get_device(self):
         return self.index
