@@ -177,9 +177,9 @@ template <int CK> __device__ __forceinline__ u32x4_t widen8(const u32x2_t &v) {
 // rows; the keys of a tile are cut into ranges of 32-key blocks, one per wavefront of each of the tile's workgroups, so that a single long
 // sequence still reaches every compute unit.  A wavefront has an LDS ring of its own (32 KB: the next block or blocks are in flight while it computes,
 // 64 KB and more per compute unit), meets nobody until its range is done, and there is no barrier in the loop.
-// Measured, bf16, 32 query and 8 key / value heads of 128: 64 tokens over up to 8192 cached each, 1.44 GB, 255 us (5.6 TB/s; a
+// Measured, bf16, 32 query and 8 key / value heads of 128: 64 tokens over up to 8192 cached each, 1.44 GB, 253 us (5.7 TB/s; a
 // large copy 5.1, reading alone 7.0); 48 over up to 16384 in 8-bit floats, 64 query heads, 1.08 GB, 230 us (4.7 TB/s: what a workgroup
-// costs besides its keys, three rounds of it; eight wavefronts with half the ring each 227); one over 1999, 8 MB, 11.5 us.
+// costs besides its keys, three rounds of it; eight wavefronts with half the ring each 227); one over 1999, 8 MB, 11.1 us.
 //
 // S^T = K Q^T and O^T += V^T P^T on 16 x 16 x 32: a lane then owns one row throughout (column lane % 16).  The rows
 // of the first product's left operand are keys in the order 8 (r / 4) + 4 t + r % 4 for tile t of two, so that a lane's
@@ -406,14 +406,15 @@ __global__ __launch_bounds__(R16_NT) void seq_attention_r16_kernel(const uint16_
             const float next = c * (top - ref) > SLACK ? top : ref;
             const float keep = __builtin_amdgcn_exp2f(c * (ref - next));
             ref = next;
+            if (blk != blk0)  // (the first block's sums are zero)
 #pragma unroll
-            for (int j = 0; j <= G::DT; j++)
+                for (int j = 0; j <= G::DT; j++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    o[j][e] *= keep;
-                    if constexpr (APART)
-                        if (j < G::DT) o_rest[j][e] *= keep;
-                }
+                    for (int e = 0; e < 4; e++) {
+                        o[j][e] *= keep;
+                        if constexpr (APART)
+                            if (j < G::DT) o_rest[j][e] *= keep;
+                    }
         }
         float p[8];
 #pragma unroll
@@ -454,10 +455,17 @@ __global__ __launch_bounds__(R16_NT) void seq_attention_r16_kernel(const uint16_
     }
 
     if constexpr (APART) {
+        float size = 0.f;
 #pragma unroll
         for (int j = 0; j < G::DT; j++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) o[j][e] += __builtin_fabsf(o[j][e]) == INFINITY ? 0.f : o_rest[j][e];
+            for (int e = 0; e < 4; e++) size = __builtin_fmaxf(size, __builtin_fabsf(o[j][e]));
+        const bool finite = __builtin_amdgcn_ballot_w64(size == INFINITY) == 0;
+#pragma unroll
+        for (int j = 0; j < G::DT; j++)
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (finite || __builtin_fabsf(o[j][e]) != INFINITY) o[j][e] += o_rest[j][e];
     }
     // ---- the four wavefronts meet: per wavefront and row (reference, sum, -, -, O) ----
     __syncthreads();
@@ -546,8 +554,8 @@ __global__ __launch_bounds__(R16_NT) void seq_attention_r16_kernel(const uint16_
 // rows each (RT = 2, 3 or 4 tiles of 16) and walk all keys of the tile, 64 to a stage of the LDS ring, 32 to a step, with the layouts of the
 // kernel above.  A fragment of K or V read from LDS feeds RT matrix instructions, which is what keeps LDS from being the bound
 // (128 bytes a cycle: a fragment per 2 RT cycles of each SIMD; the instruction takes 16).
-// Measured, bf16, causal, 32 query and 8 key / value heads of 128: 8192 tokens 547 us (1004 TFLOP/s; a matrix product of 8192^3 runs
-// at 1210); 16 prompts of up to 2048 tokens 390 us (629: a workgroup costs some 10 us besides its stages of 1.5 us, and a tile of
+// Measured, bf16, causal, 32 query and 8 key / value heads of 128: 8192 tokens 544 us (1010 TFLOP/s; a matrix product of 8192^3 runs
+// at 1210); 16 prompts of up to 2048 tokens 392 us (626: a workgroup costs some 10 us besides its stages of 1.5 us, and a tile of
 // those has 10 of them); four chunks of 512 tokens over up to 8192 285 us (758).
 //
 // P is rounded to the type for the second product, and the row sum is taken of it as rounded: the output is off by 1.3 to 1.4 times

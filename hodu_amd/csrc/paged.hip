@@ -13,7 +13,7 @@ namespace {
 // sums for itself in LDS and then takes its share of the slots, so that nothing has to pass between workgroups and one launch
 // does it.  A token's page comes from the sums (an entry that was in the table before, or the free list's), never from what
 // another workgroup may be writing.  Bound by latency: two trips to memory and a few barriers, then the slots: 8 requests of a token
-// each 4.4 us (of which a launch that does nothing is 1.8), 512 prompts of 700 000 tokens in all 8.3 us.  Running sums by halving
+// each 5.3 us (of which a launch that does nothing is 1.8), 512 prompts of 700 000 tokens in all 8.2 us.  Running sums by halving
 // strides through LDS, a barrier each, took 19 us for the latter: a wavefront sums by itself, four sums meet at one barrier.
 //
 // The sums saturate at 2^32 - 1 (a saturating sum of non-negative numbers does not depend on its order), which is beyond any
