@@ -266,7 +266,8 @@ int hodu_rocm_softmax_masked(hodu_rocm_ctx *ctx, int dtype, const void *in, void
  * after every kernel), the output is rounded once.  Takes bf16 / f16, D = 64 or 128, dense head dims, rows / offsets /
  * batch strides that are multiples of 8 elements, a positive finite scale (the row maximum is taken before the scale
  * is applied); returns HODU_ROCM_UNSUPPORTED otherwise, and the caller runs the
- * three launches (hodu_rocm_matmul_<dt>_ex with MUL_SCALAR, hodu_rocm_softmax, hodu_rocm_matmul_<dt>).
+ * three launches (hodu_rocm_matmul_<dt>_ex with MUL_SCALAR, hodu_rocm_softmax, hodu_rocm_matmul_<dt>).  Scores are told
+ * apart up to |score * scale| of some 2^22; their products with the scale no longer cancel beyond (hodu_rocm_attention_varlen's do).
  * metadata (this library's own): [nb, batch_shape (nb).., Sq, Sk, D, q_strides (nb + 2).., k_strides (nb + 2)..,
  * v_strides (nb + 2).., q_off, k_off, v_off], strides and offsets in elements, batch dims already broadcast (stride
  * 0 where an operand lacks the dim).  scale: the scalar in `dtype` (what mul_scalar receives); causal != 0 masks
